@@ -368,6 +368,128 @@ int mt_cuda_sdpa(const mt_sdpa_desc* desc, void* workspace, size_t workspace_byt
 #define MT_SDPA_PATH_TC_SHORT 4
 int mt_cuda_sdpa_path(const mt_sdpa_desc* desc);
 
+/* ---- a causal decoder's operators (no counterpart in the reference) ----------------------- */
+/*
+ * Rotary positions with several axes (time, height, width, ...) on one or two tensors of heads.
+ * Pair i of `pairs` turns by angle(i) = fp32(position[axis of i] * frequencies[i]); axis a owns the
+ * pairs below axis_end[a] (cumulative, axis_end[axes-1] == pairs).  Pair i is the elements
+ * (i, i + pairs) of the head, or (2i, 2i + 1) when `interleaved`; elements past 2 * pairs are copied.
+ *   (x, y) -> (x cos - y sin, x sin + y cos);   inverse != 0 turns back (the transpose, which is
+ *   also the gradient of the forward turn).
+ * q [B, Hq, S, D] and k [B, Hk, S, D] (Hk 0: none) with element strides (b, h, s, d); the outputs
+ * have strides of their own and may be the inputs themselves (same pointer and strides).
+ * positions: int32, token stride 1, strides for axis and batch (0 broadcasts).  f32, bf16, f16.
+ */
+#define MT_ROTARY_MAX_AXES 4
+typedef struct {
+  int64_t B, S, D, Hq, Hk;
+  int dtype, interleaved, inverse, axes;
+  int64_t pairs, axis_end[MT_ROTARY_MAX_AXES];
+  const int32_t* positions; int64_t pos_axis_stride, pos_batch_stride;
+  const float* frequencies;
+  const void* q; int64_t q_strides[4]; void* q_out; int64_t q_out_strides[4];
+  const void* k; int64_t k_strides[4]; void* k_out; int64_t k_out_strides[4];
+} mt_rotary_desc;
+int mt_cuda_rotary(const mt_rotary_desc* desc, void* stream);
+
+/*
+ * Attention with a sliding window and sinks: O = softmax(Q K^T * scale) V over the keys that a
+ * query sees.  Query i of batch entry b has position p = starts[b] + i (starts NULL: Sk - Sq + i);
+ * with n = lengths[b] (NULL: Sk; clamped to 0..Sk) it sees key j < n when
+ *   causal:      j <= p and (window == 0 or j > p - window or j < sinks)
+ *   otherwise:   window == 0 or |p - j| < window or j < sinks.
+ * A query that sees nothing gets zeros.  Keys at n and beyond may hold anything.  Q [B, H, Sq, D],
+ * K and V [B, Hkv, Sk, D], O [B, H, Sq, D] with element strides (b, h, s, d), H % Hkv == 0,
+ * D <= 256, Sq and Sk <= 2^28; f32, bf16, f16 (softmax and sums in fp32).  starts / lengths: int32 on
+ * the device; starts are clamped to +-2^29.
+ * Workspace: mt_cuda_window_attention_workspace_size (partial results when few queries split
+ * their keys over CTAs).
+ */
+typedef struct {
+  int64_t B, H, Hkv, Sq, Sk, D;
+  int dtype, causal;
+  int64_t window, sinks;
+  const int32_t* starts; const int32_t* lengths;
+  const void* q; int64_t q_strides[4];
+  const void* k; int64_t k_strides[4];
+  const void* v; int64_t v_strides[4];
+  void* o; int64_t o_strides[4];
+  double scale;
+} mt_window_attention_desc;
+size_t mt_cuda_window_attention_workspace_size(const mt_window_attention_desc* desc);
+int mt_cuda_window_attention(const mt_window_attention_desc* desc, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/*
+ * A paged key / value cache held in 4 bits.  Four contiguous arrays:
+ *   words  [num_pages, Hkv, page_size, D / 8] int32: code of channel c in bits 4 (c % 8) of word c / 8
+ *   scales [num_pages, Hkv, page_size, D / 64, 2] f16: (scale, zero) of each 64 channels
+ * for K and for V; value = zero + scale * code.  page_size is a power of two from 16 to 1024, D a
+ * multiple of 64 up to 256.  Token t of sequence b is at slot t % page_size of page
+ * block_table[b * table_stride + t / page_size] (int32).  Table entries that no call needs are not
+ * read; a needed entry outside 0..num_pages-1 makes its tokens invisible (attention), unwritten
+ * (append) or zero (read).
+ */
+typedef struct {
+  int64_t num_pages, page_size, Hkv, D;
+  int32_t* k_words; void* k_scales; int32_t* v_words; void* v_scales;
+} mt_kv_cache4;
+/* Writes T tokens per sequence at positions starts[b] .. starts[b] + T - 1 (positions below 0 or
+ * past the table are not written).  Per 64 channels, in fp32: zero = f16(min), scale =
+ * f16((max - min) * (1/15)) (both clamped to the f16 range), code = clamp(rint((x - zero) / scale), 0, 15). */
+int mt_cuda_kv_cache4_append(const mt_kv_cache4* cache, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
+                             int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream);
+/* Reads T tokens per sequence back as values: k_out and v_out [B, Hkv, T, D] with element strides. */
+int mt_cuda_kv_cache4_read(const mt_kv_cache4* cache, void* k_out, const int64_t* k_strides, void* v_out,
+                           const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
+                           int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream);
+/* Causal attention of the last Sq tokens of each sequence over the cache, with an optional window
+ * and sinks as in mt_cuda_window_attention: query i of sequence b has position lengths[b] - Sq + i
+ * and the sequence has lengths[b] keys (clamped to 0 .. max_pages * page_size).  q and o
+ * [B, H, Sq, D] in bf16 or f16. */
+typedef struct {
+  mt_kv_cache4 cache;
+  int64_t B, H, Sq;
+  int dtype;
+  int64_t window, sinks;
+  const int32_t* block_table; int64_t table_stride, max_pages;
+  const int32_t* lengths;
+  const void* q; int64_t q_strides[4];
+  void* o; int64_t o_strides[4];
+  double scale;
+} mt_kv_cache4_attention_desc;
+size_t mt_cuda_kv_cache4_attention_workspace_size(const mt_kv_cache4_attention_desc* desc);
+int mt_cuda_kv_cache4_attention(const mt_kv_cache4_attention_desc* desc, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/*
+ * Products with a weight held in 4 bits: Y [M, N] = X [M, K] W^T + bias, W[n, k] =
+ * scale[n, k / group] * (code[n, k] - 8).  words: [N, Kp / 8] int32 with Kp = K rounded up to 128;
+ * the code of column c is in bits 4 (c % 8) of word c / 8, and in each 16 words (128 columns) word
+ * w is stored at place (w % 4) * 4 + w / 4.  scales: [N, Kp / group] bf16, group 32, 64 or 128.
+ * Codes of columns past K are ignored.  X and Y have row pitches, unit column stride; f32, bf16 or
+ * f16, sums in fp32.  Workspace: mt_cuda_linear_weight4_workspace_size (many rows go through an
+ * unpacked copy of the weight and mt_cuda_gemm).
+ */
+typedef struct {
+  int64_t M, N, K, group;
+  int dtype;
+  const void* x; int64_t ldx;
+  const int32_t* words; const void* scales;
+  const void* bias; /* `dtype`, length N, or NULL */
+  void* y; int64_t ldy;
+} mt_linear_weight4_desc;
+size_t mt_cuda_linear_weight4_workspace_size(const mt_linear_weight4_desc* desc);
+int mt_cuda_linear_weight4(const mt_linear_weight4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+/* Packs a weight [N, K] (row pitch ldw; f32, bf16 or f16): scale = bf16(max|w| / 7 as
+ * max|w| * fp32(1/7)) per group, code = clamp(rint(w / scale), -8, 7) + 8, columns past K get 8. */
+int mt_cuda_weight4_pack(int32_t* words, void* scales, const void* w, int dtype, int64_t ldw, int64_t N, int64_t K,
+                         int64_t group, void* stream);
+/* Unpacks to [N, K] values of `dtype` with row pitch ldw. */
+int mt_cuda_weight4_unpack(void* w, int dtype, int64_t ldw, const int32_t* words, const void* scales, int64_t N,
+                           int64_t K, int64_t group, void* stream);
+
 /* ---- host random generator: the reference's RandomState (module.cpp:47-183) ------------- */
 /* SplitMix64 + Marsaglia-polar normal with the odd-count "spare" rule, bit-identical to
  * mtorch.manual_seed / randn / normal_ / uniform_ on contiguous float tensors.  The state is a

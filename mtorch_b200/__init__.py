@@ -14,7 +14,7 @@ import contextlib
 from . import _lib
 from . import runtime as _runtime
 from .tensor import (Size, Tensor, add, bfloat16, bool_, device, div, dtype, empty, empty_like, float16, float32,
-                     float64, from_numpy, full, int32, int64, mul, ones, sub, tensor, zeros, zeros_like)
+                     float64, from_device_memory, from_numpy, full, int32, int64, mul, ones, sub, tensor, zeros, zeros_like)
 
 float = float32  # noqa: A001  (torch-style aliases)
 half = float16
@@ -24,6 +24,8 @@ bool = bool_  # noqa: A001
 from .random import Generator, default_generator, initial_seed, manual_seed, rand, randn, randn_like
 from .ops import (addmm, baddbmm, bmm, cat, conv2d, gelu, group_norm, layer_norm, linear, log_softmax, matmul, mm,
                   scaled_dot_product_attention, silu, softmax)
+from .decoding import (KVCache4, Weight4, kv_cache_append, kv_cache_attention, kv_cache_read, linear_weight4,
+                       rotary_embedding, rotary_frequencies, window_attention)
 from . import nn
 
 channels_last = "channels_last"

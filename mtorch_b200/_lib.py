@@ -69,6 +69,64 @@ class SdpaDesc(C.Structure):
     ]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [
+        ("B", I64), ("S", I64), ("D", I64), ("Hq", I64), ("Hk", I64),
+        ("dtype", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("axes", C.c_int),
+        ("pairs", I64), ("axis_end", I64_4),
+        ("positions", VP), ("pos_axis_stride", I64), ("pos_batch_stride", I64),
+        ("frequencies", VP),
+        ("q", VP), ("q_strides", I64_4), ("q_out", VP), ("q_out_strides", I64_4),
+        ("k", VP), ("k_strides", I64_4), ("k_out", VP), ("k_out_strides", I64_4),
+    ]
+
+
+class WindowAttentionDesc(C.Structure):
+    _fields_ = [
+        ("B", I64), ("H", I64), ("Hkv", I64), ("Sq", I64), ("Sk", I64), ("D", I64),
+        ("dtype", C.c_int), ("causal", C.c_int),
+        ("window", I64), ("sinks", I64),
+        ("starts", VP), ("lengths", VP),
+        ("q", VP), ("q_strides", I64_4),
+        ("k", VP), ("k_strides", I64_4),
+        ("v", VP), ("v_strides", I64_4),
+        ("o", VP), ("o_strides", I64_4),
+        ("scale", C.c_double),
+    ]
+
+
+class KvCache4Desc(C.Structure):
+    _fields_ = [
+        ("num_pages", I64), ("page_size", I64), ("Hkv", I64), ("D", I64),
+        ("k_words", VP), ("k_scales", VP), ("v_words", VP), ("v_scales", VP),
+    ]
+
+
+class KvCache4AttentionDesc(C.Structure):
+    _fields_ = [
+        ("cache", KvCache4Desc),
+        ("B", I64), ("H", I64), ("Sq", I64),
+        ("dtype", C.c_int),
+        ("window", I64), ("sinks", I64),
+        ("block_table", VP), ("table_stride", I64), ("max_pages", I64),
+        ("lengths", VP),
+        ("q", VP), ("q_strides", I64_4),
+        ("o", VP), ("o_strides", I64_4),
+        ("scale", C.c_double),
+    ]
+
+
+class LinearWeight4Desc(C.Structure):
+    _fields_ = [
+        ("M", I64), ("N", I64), ("K", I64), ("group", I64),
+        ("dtype", C.c_int),
+        ("x", VP), ("ldx", I64),
+        ("words", VP), ("scales", VP),
+        ("bias", VP),
+        ("y", VP), ("ldy", I64),
+    ]
+
+
 class RngState(C.Structure):
     _fields_ = [("state", C.c_uint64), ("has_spare", C.c_int32), ("spare", C.c_double)]
 
@@ -145,6 +203,19 @@ SIGNATURES = {
     "mt_cuda_sdpa_workspace_size": (C.c_size_t, [C.POINTER(SdpaDesc)]),
     "mt_cuda_sdpa": (C.c_int, [C.POINTER(SdpaDesc), VP, C.c_size_t, VP]),
     "mt_cuda_sdpa_path": (C.c_int, [C.POINTER(SdpaDesc)]),
+    "mt_cuda_rotary": (C.c_int, [C.POINTER(RotaryDesc), VP]),
+    "mt_cuda_window_attention_workspace_size": (C.c_size_t, [C.POINTER(WindowAttentionDesc)]),
+    "mt_cuda_window_attention": (C.c_int, [C.POINTER(WindowAttentionDesc), VP, C.c_size_t, VP]),
+    "mt_cuda_kv_cache4_append": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
+                                           I64, VP, VP]),
+    "mt_cuda_kv_cache4_read": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
+                                         I64, VP, VP]),
+    "mt_cuda_kv_cache4_attention_workspace_size": (C.c_size_t, [C.POINTER(KvCache4AttentionDesc)]),
+    "mt_cuda_kv_cache4_attention": (C.c_int, [C.POINTER(KvCache4AttentionDesc), VP, C.c_size_t, VP]),
+    "mt_cuda_linear_weight4_workspace_size": (C.c_size_t, [C.POINTER(LinearWeight4Desc)]),
+    "mt_cuda_linear_weight4": (C.c_int, [C.POINTER(LinearWeight4Desc), VP, C.c_size_t, VP]),
+    "mt_cuda_weight4_pack": (C.c_int, [VP, VP, VP, C.c_int, I64, I64, I64, I64, VP]),
+    "mt_cuda_weight4_unpack": (C.c_int, [VP, C.c_int, I64, VP, VP, I64, I64, I64, VP]),
     "mt_rng_seed": (None, [C.POINTER(RngState), C.c_uint64]),
     "mt_rng_fill_normal": (None, [C.POINTER(RngState), VP, C.c_int, I64, C.c_double, C.c_double]),
     "mt_rng_fill_uniform": (None, [C.POINTER(RngState), VP, C.c_int, I64, C.c_double, C.c_double]),

@@ -321,6 +321,61 @@ int mt_cuda_sdpa(const mt_sdpa_desc* desc, void* workspace, size_t workspace_byt
   return run_sdpa(*desc, workspace, workspace_bytes, S(stream));
 }
 
+// ---- a causal decoder's operators ------------------------------------------------------------
+int mt_cuda_rotary(const mt_rotary_desc* desc, void* stream) {
+  if (!desc) return fail(MT_ERR_INVALID, "rotary: null descriptor");
+  return run_rotary(*desc, S(stream));
+}
+
+size_t mt_cuda_window_attention_workspace_size(const mt_window_attention_desc* desc) {
+  return desc ? window_attention_workspace(*desc) : 0;
+}
+int mt_cuda_window_attention(const mt_window_attention_desc* desc, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  if (!desc) return fail(MT_ERR_INVALID, "window_attention: null descriptor");
+  return run_window_attention(*desc, workspace, workspace_bytes, S(stream));
+}
+
+int mt_cuda_kv_cache4_append(const mt_kv_cache4* cache, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
+                             int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream) {
+  if (!cache || !k_strides || !v_strides) return fail(MT_ERR_INVALID, "kv_cache4_append: null argument");
+  return run_kv_cache4_append(*cache, k, k_strides, v, v_strides, dtype, B, T, block_table, table_stride, max_pages,
+                              starts, S(stream));
+}
+int mt_cuda_kv_cache4_read(const mt_kv_cache4* cache, void* k_out, const int64_t* k_strides, void* v_out,
+                           const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
+                           int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream) {
+  if (!cache || !k_strides || !v_strides) return fail(MT_ERR_INVALID, "kv_cache4_read: null argument");
+  return run_kv_cache4_read(*cache, k_out, k_strides, v_out, v_strides, dtype, B, T, block_table, table_stride,
+                            max_pages, starts, S(stream));
+}
+size_t mt_cuda_kv_cache4_attention_workspace_size(const mt_kv_cache4_attention_desc* desc) {
+  return desc ? kv_cache4_attention_workspace(*desc) : 0;
+}
+int mt_cuda_kv_cache4_attention(const mt_kv_cache4_attention_desc* desc, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (!desc) return fail(MT_ERR_INVALID, "kv_cache4_attention: null descriptor");
+  return run_kv_cache4_attention(*desc, workspace, workspace_bytes, S(stream));
+}
+
+size_t mt_cuda_linear_weight4_workspace_size(const mt_linear_weight4_desc* desc) {
+  return desc ? linear_weight4_workspace(*desc) : 0;
+}
+int mt_cuda_linear_weight4(const mt_linear_weight4_desc* desc, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (!desc) return fail(MT_ERR_INVALID, "linear_weight4: null descriptor");
+  return run_linear_weight4(*desc, workspace, workspace_bytes, S(stream));
+}
+int mt_cuda_weight4_pack(int32_t* words, void* scales, const void* w, int dtype, int64_t ldw, int64_t N, int64_t K,
+                         int64_t group, void* stream) {
+  return run_weight4_pack(words, scales, w, dtype, ldw, N, K, group, S(stream));
+}
+int mt_cuda_weight4_unpack(void* w, int dtype, int64_t ldw, const int32_t* words, const void* scales, int64_t N,
+                           int64_t K, int64_t group, void* stream) {
+  return run_weight4_unpack(w, dtype, ldw, words, scales, N, K, group, S(stream));
+}
+
 // ---- host generator: SplitMix64 + Marsaglia polar, as the reference's RandomState ----------
 static uint64_t rng_next(mt_rng_state* r) {
   r->state += 0x9E3779B97F4A7C15ULL;

@@ -1,0 +1,209 @@
+// Writing to and reading from the paged 4-bit key / value cache (attention over it:
+// window_attention.cu).
+//
+// One thread per word of 8 channels, 8 neighbouring threads per group of 64 channels: the group's
+// minimum and maximum come from three shuffles.  Bound by memory: the values are read once and 36
+// bytes are written per 64 channels.
+#include "runtime.h"
+
+namespace mt {
+
+struct Cache4Params {
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages, page_shift, num_pages;
+  int Hkv, D, T;
+  int64_t items;  // B * T * Hkv * D / 8
+  const int32_t* starts;
+  int32_t* words[2];
+  __half2* scales[2];  // (scale, zero)
+  const void* in[2];
+  void* out[2];
+  int64_t st[2][4];
+  bool vec;  // 8 channels are one aligned vector (16-bit types: 16 bytes, fp32: two of 16)
+};
+
+// Index of (token t of sequence b, head h) in units of heads' rows, -1 where it has no place.
+__device__ __forceinline__ int64_t cache4_row(const Cache4Params& p, int64_t b, int h, int t) {
+  const int64_t at = (int64_t)p.starts[b] + t;
+  const int64_t pi = at >> p.page_shift;
+  if (at < 0 || pi >= p.max_pages) return -1;
+  const int page = p.table[b * p.table_stride + pi];
+  if (page < 0 || page >= p.num_pages) return -1;
+  const int slot = (int)(at & ((1 << p.page_shift) - 1));
+  return (((int64_t)page * p.Hkv + h) << p.page_shift) + slot;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* src, int64_t st, bool vec, float (&x)[8]) {
+  if (vec) {
+    uint4 raw[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(src)[i];
+    const T* v = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[i * st]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int kv = blockIdx.y;
+  const int W = p.D / 8;
+  const bool live = idx < p.items;  // whole groups of 8 threads are live or not
+  const int64_t i = live ? idx : 0;
+  const int w = (int)(i % W);
+  int64_t r = i / W;
+  const int h = (int)(r % p.Hkv);
+  r /= p.Hkv;
+  const int t = (int)(r % p.T);
+  const int64_t b = r / p.T;
+  const int64_t row = live ? cache4_row(p, b, h, t) : -1;
+  const T* src = static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
+                 (int64_t)w * 8 * p.st[kv][3];
+  float x[8];
+  load8<T>(src, p.st[kv][3], p.vec, x);
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) {
+    lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, x[j]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (row < 0) return;
+  const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+  const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
+  const float z = __half2float(zero), s = __half2float(scale);
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // the division is the definition's own rounding; rint ties go to the even code
+    const float c = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f) : 0.f;
+    word |= (uint32_t)c << (4 * j);
+  }
+  p.words[kv][row * W + w] = (int32_t)word;
+  if ((w & 7) == 0) p.scales[kv][row * (p.D / 64) + (w >> 3)] = __halves2half2(scale, zero);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int kv = blockIdx.y;
+  if (idx >= p.items) return;
+  const int W = p.D / 8;
+  const int w = (int)(idx % W);
+  int64_t r = idx / W;
+  const int t = (int)(r % p.T);
+  r /= p.T;
+  const int h = (int)(r % p.Hkv);
+  const int64_t b = r / p.Hkv;
+  const int64_t row = cache4_row(p, b, h, t);
+  uint32_t word = 0;
+  float s = 0.f, z = 0.f;
+  if (row >= 0) {
+    word = (uint32_t)p.words[kv][row * W + w];
+    const __half2 sz = p.scales[kv][row * (p.D / 64) + (w >> 3)];
+    s = __low2float(sz);
+    z = __high2float(sz);
+  }
+  T* dst = static_cast<T*>(p.out[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
+           (int64_t)w * 8 * p.st[kv][3];
+  alignas(16) T v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(fmaf((float)((word >> (4 * j)) & 15u), s, z));
+  if (p.vec) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+      reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(v)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dst[j * p.st[kv][3]] = v[j];
+  }
+}
+
+int validate_kv_cache4(const mt_kv_cache4& c) {
+  if (c.num_pages < 0 || c.num_pages > INT32_MAX || c.Hkv <= 0 || c.Hkv > 65535)
+    return fail(MT_ERR_INVALID, "kv_cache4: bad sizes");
+  if (c.page_size < 16 || c.page_size > 1024 || (c.page_size & (c.page_size - 1)))
+    return fail(MT_ERR_INVALID, "kv_cache4: page_size %lld is not a power of two from 16 to 1024",
+                (long long)c.page_size);
+  if (c.D < 64 || c.D > 256 || c.D % 64)
+    return fail(MT_ERR_INVALID, "kv_cache4: head dim %lld is not a multiple of 64 up to 256", (long long)c.D);
+  if (c.num_pages && (!c.k_words || !c.k_scales || !c.v_words || !c.v_scales))
+    return fail(MT_ERR_INVALID, "kv_cache4: null cache array");
+  for (const void* a : {(const void*)c.k_words, (const void*)c.k_scales, (const void*)c.v_words,
+                        (const void*)c.v_scales})
+    if ((uintptr_t)a % 16) return fail(MT_ERR_INVALID, "kv_cache4: cache arrays have to be 16-byte aligned");
+  return MT_OK;
+}
+
+static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v,
+                         const int64_t* vs, int dtype, int64_t B, int64_t T, const int32_t* table,
+                         int64_t table_stride, int64_t max_pages, const int32_t* starts, const char* what) {
+  int rc = validate_kv_cache4(c);
+  if (rc) return rc;
+  if (dtype != MT_F32 && dtype != MT_BF16 && dtype != MT_F16) return fail(MT_ERR_UNSUPPORTED, "%s: dtype", what);
+  if (B < 0 || T < 0 || T > INT32_MAX || max_pages < 0 || max_pages > INT32_MAX)
+    return fail(MT_ERR_INVALID, "%s: bad sizes", what);
+  if (B && T && (!k || !v || !starts || (max_pages && !table))) return fail(MT_ERR_INVALID, "%s: null operand", what);
+  p.table = table; p.table_stride = table_stride; p.max_pages = (int)max_pages;
+  p.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
+  p.num_pages = (int)c.num_pages;
+  p.Hkv = (int)c.Hkv; p.D = (int)c.D; p.T = (int)T;
+  p.items = B * T * c.Hkv * (c.D / 8);
+  p.starts = starts;
+  p.words[0] = c.k_words; p.words[1] = c.v_words;
+  p.scales[0] = static_cast<__half2*>(c.k_scales); p.scales[1] = static_cast<__half2*>(c.v_scales);
+  const int es = dtype_size(dtype);
+  p.vec = true;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i ? vs : ks;
+    for (int j = 0; j < 4; ++j) p.st[i][j] = s[j];
+    p.vec = p.vec && s[3] == 1 && (uintptr_t)(i ? v : k) % 16 == 0;
+    for (int j = 0; j < 3; ++j) p.vec = p.vec && (s[j] * es) % 16 == 0;
+  }
+  if ((p.items + 255) / 256 > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "%s: too many elements", what);
+  return MT_OK;
+}
+
+int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
+                         int dtype, int64_t B, int64_t T, const int32_t* table, int64_t table_stride,
+                         int64_t max_pages, const int32_t* starts, cudaStream_t st) {
+  Cache4Params p{};
+  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_append");
+  if (rc || p.items == 0) return rc;
+  p.in[0] = k; p.in[1] = v;
+  dim3 grid((unsigned)((p.items + 255) / 256), 2);
+  switch (dtype) {
+    case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
+    case MT_BF16: cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
+    default: cache4_append_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+  }
+  return check_launch("kv_cache4_append");
+}
+
+int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* v, const int64_t* vs, int dtype,
+                       int64_t B, int64_t T, const int32_t* table, int64_t table_stride, int64_t max_pages,
+                       const int32_t* starts, cudaStream_t st) {
+  Cache4Params p{};
+  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_read");
+  if (rc || p.items == 0) return rc;
+  p.out[0] = k; p.out[1] = v;
+  dim3 grid((unsigned)((p.items + 255) / 256), 2);
+  switch (dtype) {
+    case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;
+    case MT_BF16: cache4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
+    default: cache4_read_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+  }
+  return check_launch("kv_cache4_read");
+}
+
+}  // namespace mt

@@ -104,6 +104,26 @@ int run_sdpa(const mt_sdpa_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
 int validate_sdpa_desc(const mt_sdpa_desc& d);
 int sdpa_tc_path(const mt_sdpa_desc& d);
 
+// rotary.cu, window_attention.cu, kv_cache4.cu, linear4.cu
+int run_rotary(const mt_rotary_desc& d, cudaStream_t st);
+size_t window_attention_workspace(const mt_window_attention_desc& d);
+int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+int validate_kv_cache4(const mt_kv_cache4& c);
+int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
+                         int dtype, int64_t B, int64_t T, const int32_t* table, int64_t table_stride,
+                         int64_t max_pages, const int32_t* starts, cudaStream_t st);
+int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* v, const int64_t* vs, int dtype,
+                       int64_t B, int64_t T, const int32_t* table, int64_t table_stride, int64_t max_pages,
+                       const int32_t* starts, cudaStream_t st);
+size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d);
+int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+size_t linear_weight4_workspace(const mt_linear_weight4_desc& d);
+int run_linear_weight4(const mt_linear_weight4_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+int run_weight4_pack(int32_t* words, void* scales, const void* w, int dtype, int64_t ldw, int64_t N, int64_t K,
+                     int64_t group, cudaStream_t st);
+int run_weight4_unpack(void* w, int dtype, int64_t ldw, const int32_t* words, const void* scales, int64_t N, int64_t K,
+                       int64_t group, cudaStream_t st);
+
 // Per-translation-unit device status readers (see g_device_error).
 int read_status_gemm(int clear);
 int run_wait_timeout_selftest(long long budget_cycles, cudaStream_t st);

@@ -1,0 +1,387 @@
+// Attention with a sliding window and sinks, over 16-bit / fp32 keys and values or over the paged
+// 4-bit cache.
+//
+// One pass over the keys with the running maximum and sum of the softmax in fp32:
+//   m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' = o 2^(m - m') + 2^(s - m') v.
+// Only blocks of keys that a row of the tile can see are visited.  Few rows leave most of the GPU
+// idle, so their keys are split over CTAs; the partial (m, l, o) go to the workspace and are joined
+// by a second kernel.
+#include <algorithm>
+
+#include "window_attention.cuh"
+
+namespace mt {
+
+constexpr int kRowTile = 4;    // rows per CTA of attn_rows_kernel
+constexpr int kRowBlock = 16;  // keys per step of a warp
+
+enum { KV_ALIGNED = 0, KV_STRIDED = 1, KV_PAGED4 = 2 };
+
+// One CTA (4 warps) = kRowTile rows of one (batch entry, key head) and one share of their keys.
+// A group of 8 lanes works on one key: a lane holds 4 channels of every 32.
+template <typename T, int DCH, int KIND>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
+  constexpr int DP = DCH * 32;
+  __shared__ float sq[kRowTile][DP];
+  __shared__ float so[4][kRowTile][DP];
+  __shared__ float2 sml[4][kRowTile];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7, grp = lane >> 3;
+  const int bk = blockIdx.y, b = bk / p.Hkv, hk = bk % p.Hkv;
+  const int r0 = blockIdx.z * kRowTile, nr = min(kRowTile, p.rows - r0);
+  const SeqPos sp = seq_pos(p, b, KIND == KV_PAGED4);
+
+  for (int i = threadIdx.x; i < kRowTile * DP; i += 128) {
+    const int r = i / DP, d = i % DP;
+    float x = 0.f;
+    if (r < nr && d < p.D) {
+      const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
+      x = to_f32<T>(static_cast<const T*>(p.q)[b * p.qs[0] + h * p.qs[1] + qi * p.qs[2] + d * p.qs[3]]);
+    }
+    sq[r][d] = x * p.scale_log2;
+  }
+  __syncthreads();
+
+  RowKeys rk[kRowTile];
+#pragma unroll
+  for (int r = 0; r < kRowTile; ++r) rk[r] = row_keys(p, sp, sp.start + (r0 + min(r, nr - 1)) / p.g);
+  const BlockList bl = block_list<kRowBlock>(p, sp, sp.start + r0 / p.g, sp.start + (r0 + nr - 1) / p.g);
+  const int per = (bl.count + p.splits - 1) / p.splits;
+  const int i0 = blockIdx.x * per, i1 = min(bl.count, i0 + per);
+
+  float m[kRowTile], l[kRowTile], o[kRowTile][DCH][4];
+#pragma unroll
+  for (int r = 0; r < kRowTile; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DCH; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[r][c][j] = 0.f;
+  }
+
+  for (int i = i0 + warp; i < i1; i += 4) {
+    const int k0 = bl.block(i) * kRowBlock;
+    int64_t page_row = 0;
+    bool here = true;
+    if (KIND == KV_PAGED4) {
+      const int page = p.table[b * p.table_stride + (k0 >> p.page_shift)];
+      here = page >= 0 && page < p.num_pages;
+      page_row = (((int64_t)(here ? page : 0) * p.Hkv + hk) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
+    }
+#pragma unroll 1
+    for (int it = 0; it < kRowBlock / 4; ++it) {
+      const int kk = it * 4 + grp, key = k0 + kk;
+      const bool live = here && key < sp.n;
+      auto load = [&](int which, float (&x)[DCH][4]) {
+#pragma unroll
+        for (int c = 0; c < DCH; ++c) {
+          const int d = c * 32 + l8 * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[c][j] = 0.f;
+          if (!live || d >= p.D) continue;
+          if (KIND == KV_PAGED4) {
+            const int64_t row = page_row + kk;
+            const uint32_t w = p.words[which][row * (p.D / 8) + d / 8] >> ((d & 4) * 4);
+            const __half2 sz = p.scales[which][row * (p.D / 64) + d / 64];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              x[c][j] = fmaf((float)((w >> (4 * j)) & 15u), __low2float(sz), __high2float(sz));
+          } else {
+            const int64_t* s = which ? p.vs : p.ks;
+            const T* src = static_cast<const T*>(which ? p.v : p.k) + b * s[0] + hk * s[1] + key * s[2];
+            if (KIND == KV_ALIGNED) {
+              alignas(16) T raw[4];
+              if (sizeof(T) == 4) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + d);
+              else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src + d);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[c][j] = to_f32<T>(raw[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (d + j < p.D) x[c][j] = to_f32<T>(src[(d + j) * s[3]]);
+            }
+          }
+        }
+      };
+      float kf[DCH][4], vf[DCH][4];
+      load(0, kf);
+      load(1, vf);
+#pragma unroll
+      for (int r = 0; r < kRowTile; ++r) {
+        if (r >= nr) break;
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < DCH; ++c) {
+          const float4 qv = *reinterpret_cast<const float4*>(&sq[r][c * 32 + l8 * 4]);
+          s = fmaf(qv.x, kf[c][0], s);
+          s = fmaf(qv.y, kf[c][1], s);
+          s = fmaf(qv.z, kf[c][2], s);
+          s = fmaf(qv.w, kf[c][3], s);
+        }
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        if (!live || !rk[r].sees(key)) continue;
+        const float mn = fmaxf(m[r], s);
+        const float corr = exp2f(m[r] - mn), e = exp2f(s - mn);
+        m[r] = mn;
+        l[r] = fmaf(l[r], corr, e);
+#pragma unroll
+        for (int c = 0; c < DCH; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[r][c][j] = fmaf(o[r][c][j], corr, e * vf[c][j]);
+      }
+    }
+  }
+
+  // join the four key groups of the warp, then the four warps
+#pragma unroll
+  for (int r = 0; r < kRowTile; ++r) {
+    float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+    float ls = l[r] * f;
+    ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+    ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+    if (lane == 0) sml[warp][r] = make_float2(top, ls);
+#pragma unroll
+    for (int c = 0; c < DCH; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = m[r] == -INFINITY ? 0.f : o[r][c][j] * f;
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (grp == 0) so[warp][r][c * 32 + l8 * 4 + j] = x;
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nr * DP; i += 128) {
+    const int r = i / DP, d = i % DP;
+    if (d >= p.D) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][r].x);
+    float ls = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (sml[w][r].x != -INFINITY) {
+        const float f = exp2f(sml[w][r].x - top);
+        ls = fmaf(sml[w][r].y, f, ls);
+        x = fmaf(so[w][r][d], f, x);
+      }
+    if (p.splits > 1) {
+      const int64_t row = ((int64_t)blockIdx.x * p.B * p.Hkv + bk) * p.rows + r0 + r;
+      p.part_o[row * p.D + d] = x;
+      if (d == 0) p.part_ml[row] = make_float2(top, ls);
+    } else {
+      const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
+      static_cast<T*>(p.o)[b * p.os[0] + h * p.os[1] + qi * p.os[2] + d * p.os[3]] =
+          from_f32<T>(ls > 0.f ? x / ls : 0.f);
+    }
+  }
+}
+
+// One warp joins the shares of one row.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+  const int64_t total = (int64_t)p.B * p.Hkv * p.rows;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= total) return;
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[s * total + row].x);
+  top = warp_max(top);
+  float ls = 0.f;
+  for (int s = lane; s < p.splits; s += 32) {
+    const float2 ml = p.part_ml[s * total + row];
+    if (ml.x != -INFINITY) ls = fmaf(ml.y, exp2f(ml.x - top), ls);
+  }
+  ls = warp_sum(ls);
+  const int64_t bk = row / p.rows;
+  const int r = (int)(row - bk * p.rows);
+  const int b = (int)(bk / p.Hkv), hk = (int)(bk % p.Hkv);
+  T* dst = static_cast<T*>(p.o) + b * p.os[0] + (hk * p.g + r % p.g) * p.os[1] + (r / p.g) * p.os[2];
+  for (int d = lane; d < p.D; d += 32) {
+    float x = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float ms = p.part_ml[s * total + row].x;
+      if (ms != -INFINITY) x = fmaf(p.part_o[(s * total + row) * p.D + d], exp2f(ms - top), x);
+    }
+    dst[d * p.os[3]] = from_f32<T>(ls > 0.f ? x / ls : 0.f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+
+// Keys that one row can see at most.
+static int64_t span_keys(int64_t Sk, int64_t Sq, int causal, int64_t window, int64_t sinks) {
+  if (window <= 0) return Sk;
+  return std::min(Sk, (causal ? window : 2 * window - 1) + Sq - 1 + sinks + 2 * kRowBlock);
+}
+
+// Shares of the keys: enough CTAs to fill the GPU a few times, each with at least 8 blocks of keys.
+static int choose_splits(int64_t ctas, int64_t keys) {
+  const int64_t want = (4LL * num_sms() + ctas - 1) / ctas;
+  const int64_t most = std::max<int64_t>(1, keys / (8 * kRowBlock));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 512));
+}
+
+static size_t part_bytes(int splits, int64_t rows, int64_t D) {
+  if (splits <= 1) return 0;
+  return align_up((size_t)splits * rows * sizeof(float2), 256) + (size_t)splits * rows * D * sizeof(float);
+}
+
+static int rows_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int causal, int64_t window,
+                       int64_t sinks) {
+  const int64_t tiles = (Sq * (H / Hkv) + kRowTile - 1) / kRowTile;
+  return choose_splits(B * Hkv * tiles, span_keys(Sk, Sq, causal, window, sinks));
+}
+
+static void bind_workspace(AttnParams& p, void* ws) {
+  const size_t rows = (size_t)p.B * p.Hkv * p.rows;
+  p.part_ml = static_cast<float2*>(ws);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + align_up((size_t)p.splits * rows * sizeof(float2), 256));
+}
+
+template <typename T>
+static int join_launch(const AttnParams& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
+  attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p);
+  return check_launch("attention_join");
+}
+
+template <typename T, int KIND>
+static int rows_launch(const AttnParams& p, cudaStream_t st) {
+  const int64_t tiles = (p.rows + kRowTile - 1) / kRowTile;
+  if ((int64_t)p.B * p.Hkv > 65535 || tiles > 65535)
+    return fail(MT_ERR_UNSUPPORTED, "window_attention: batch * key heads or rows past the grid");
+  dim3 grid((unsigned)p.splits, (unsigned)(p.B * p.Hkv), (unsigned)tiles);
+  const int dch = (p.D + 31) / 32;
+  if (dch <= 2) attn_rows_kernel<T, 2, KIND><<<grid, 128, 0, st>>>(p);
+  else if (dch <= 4) attn_rows_kernel<T, 4, KIND><<<grid, 128, 0, st>>>(p);
+  else attn_rows_kernel<T, 8, KIND><<<grid, 128, 0, st>>>(p);
+  int rc = check_launch("attention_rows");
+  if (rc || p.splits == 1) return rc;
+  return join_launch<T>(p, st);
+}
+
+static int check_common(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window,
+                        int64_t sinks, double scale, const char* what) {
+  if (B < 0 || H <= 0 || Hkv <= 0 || Sq < 0 || Sk < 0 || D <= 0 || window < 0 || sinks < 0)
+    return fail(MT_ERR_INVALID, "%s: bad sizes", what);
+  if (H % Hkv) return fail(MT_ERR_INVALID, "%s: %lld heads are no multiple of %lld key heads", what, (long long)H,
+                           (long long)Hkv);
+  if (D > 256) return fail(MT_ERR_UNSUPPORTED, "%s: head dim > 256", what);
+  if (!(scale == scale) || scale > 1e30 || scale < -1e30) return fail(MT_ERR_INVALID, "%s: scale", what);
+  if (Sq > kMaxKeys || Sk > kMaxKeys || B > INT32_MAX || Sq * (H / Hkv) > INT32_MAX / 2)
+    return fail(MT_ERR_UNSUPPORTED, "%s: sizes past the kernels' range", what);
+  return MT_OK;
+}
+
+static int clamp_window(int64_t w) { return w <= 0 || w >= kNoWindow ? kNoWindow : (int)w; }
+
+static int validate_window(const mt_window_attention_desc& d) {
+  int rc = check_common(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.D, d.window, d.sinks, d.scale, "window_attention");
+  if (rc) return rc;
+  if (d.dtype != MT_F32 && d.dtype != MT_BF16 && d.dtype != MT_F16)
+    return fail(MT_ERR_UNSUPPORTED, "window_attention: dtype");
+  if (d.B && d.Sq && (!d.q || !d.o || (d.Sk && (!d.k || !d.v))))
+    return fail(MT_ERR_INVALID, "window_attention: null operand");
+  return MT_OK;
+}
+
+size_t window_attention_workspace(const mt_window_attention_desc& d) {
+  if (validate_window(d) || d.B == 0 || d.Sq == 0) return 0;
+  return part_bytes(rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks), d.B * d.H * d.Sq, d.D);
+}
+
+// 4 channels are one aligned vector
+static bool aligned4(const void* base, const int64_t* s, int64_t D, int es) {
+  if (s[3] != 1 || D % 4 || (uintptr_t)base % (4 * es)) return false;
+  return s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+}
+
+template <typename T>
+static int window_dispatch(const mt_window_attention_desc& d, const AttnParams& p, cudaStream_t st) {
+  if (aligned4(d.k, d.k_strides, d.D, sizeof(T)) && aligned4(d.v, d.v_strides, d.D, sizeof(T)))
+    return rows_launch<T, KV_ALIGNED>(p, st);
+  return rows_launch<T, KV_STRIDED>(p, st);
+}
+
+int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
+  int rc = validate_window(d);
+  if (rc || d.B == 0 || d.Sq == 0) return rc;
+  AttnParams p{};
+  p.B = (int)d.B; p.H = (int)d.H; p.Hkv = (int)d.Hkv; p.g = (int)(d.H / d.Hkv);
+  p.Sq = (int)d.Sq; p.Sk = (int)d.Sk; p.D = (int)d.D; p.rows = p.g * p.Sq;
+  p.causal = d.causal != 0;
+  p.window = clamp_window(d.window);
+  p.sinks = (int)std::min<int64_t>(d.sinks, kNoWindow);
+  p.scale_log2 = (float)(d.scale * 1.4426950408889634);
+  p.starts = d.starts; p.lengths = d.lengths;
+  p.q = d.q; p.k = d.k; p.v = d.v; p.o = d.o;
+  for (int i = 0; i < 4; ++i) {
+    p.qs[i] = d.q_strides[i]; p.ks[i] = d.k_strides[i]; p.vs[i] = d.v_strides[i]; p.os[i] = d.o_strides[i];
+  }
+  p.splits = rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks);
+  if (ws_bytes < window_attention_workspace(d) || (p.splits > 1 && !ws))
+    return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
+  bind_workspace(p, ws);
+  switch (d.dtype) {
+    case MT_F32: return window_dispatch<float>(d, p, st);
+    case MT_BF16: return window_dispatch<__nv_bfloat16>(d, p, st);
+    default: return window_dispatch<__half>(d, p, st);
+  }
+}
+
+static int validate_cache_attention(const mt_kv_cache4_attention_desc& d) {
+  int rc = validate_kv_cache4(d.cache);
+  if (rc) return rc;
+  if (d.max_pages < 0 || d.max_pages > INT32_MAX) return fail(MT_ERR_INVALID, "kv_cache4_attention: max_pages");
+  rc = check_common(d.B, d.H, d.cache.Hkv, d.Sq, d.max_pages * d.cache.page_size, d.cache.D, d.window, d.sinks, d.scale,
+                    "kv_cache4_attention");
+  if (rc) return rc;
+  if (d.dtype != MT_BF16 && d.dtype != MT_F16)
+    return fail(MT_ERR_UNSUPPORTED, "kv_cache4_attention: queries are bf16 or f16");
+  if (d.B && d.Sq && (!d.q || !d.o || !d.lengths || (d.max_pages && !d.block_table)))
+    return fail(MT_ERR_INVALID, "kv_cache4_attention: null operand");
+  return MT_OK;
+}
+
+size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d) {
+  if (validate_cache_attention(d) || d.B == 0 || d.Sq == 0) return 0;
+  return part_bytes(rows_splits(d.B, d.H, d.cache.Hkv, d.Sq, d.max_pages * d.cache.page_size, 1, d.window, d.sinks),
+                    d.B * d.H * d.Sq, d.cache.D);
+}
+
+int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
+  int rc = validate_cache_attention(d);
+  if (rc || d.B == 0 || d.Sq == 0) return rc;
+  AttnParams p{};
+  p.B = (int)d.B; p.H = (int)d.H; p.Hkv = (int)d.cache.Hkv; p.g = (int)(d.H / d.cache.Hkv);
+  p.Sq = (int)d.Sq; p.Sk = (int)(d.max_pages * d.cache.page_size); p.D = (int)d.cache.D; p.rows = p.g * p.Sq;
+  p.causal = 1;
+  p.window = clamp_window(d.window);
+  p.sinks = (int)std::min<int64_t>(d.sinks, kNoWindow);
+  p.scale_log2 = (float)(d.scale * 1.4426950408889634);
+  p.lengths = d.lengths;
+  p.q = d.q; p.o = d.o;
+  for (int i = 0; i < 4; ++i) {
+    p.qs[i] = d.q_strides[i]; p.os[i] = d.o_strides[i];
+  }
+  p.words[0] = reinterpret_cast<const uint32_t*>(d.cache.k_words);
+  p.words[1] = reinterpret_cast<const uint32_t*>(d.cache.v_words);
+  p.scales[0] = static_cast<const __half2*>(d.cache.k_scales);
+  p.scales[1] = static_cast<const __half2*>(d.cache.v_scales);
+  p.table = d.block_table; p.table_stride = d.table_stride;
+  p.num_pages = (int)d.cache.num_pages;
+  p.page_shift = __builtin_ctzll((unsigned long long)d.cache.page_size);
+  p.splits = rows_splits(d.B, d.H, d.cache.Hkv, d.Sq, p.Sk, 1, d.window, d.sinks);
+  if (ws_bytes < kv_cache4_attention_workspace(d) || (p.splits > 1 && !ws))
+    return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
+  bind_workspace(p, ws);
+  if (d.dtype == MT_BF16) return rows_launch<__nv_bfloat16, KV_PAGED4>(p, st);
+  return rows_launch<__half, KV_PAGED4>(p, st);
+}
+
+}  // namespace mt

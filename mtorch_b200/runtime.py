@@ -73,6 +73,21 @@ class DeviceBuffer:
             self.ptr = None
 
 
+class ExternalBuffer:
+    """Device bytes of another owner: `owner` (kept alive with the views) holds the memory."""
+
+    __slots__ = ("ptr", "nbytes", "device", "owner", "__weakref__")
+
+    def __init__(self, ptr: int, nbytes: int, device: int, owner):
+        self.ptr, self.nbytes, self.device, self.owner = int(ptr), int(nbytes), device, owner
+
+    def data_ptr(self) -> int:
+        return self.ptr
+
+    def numel(self) -> int:
+        return self.nbytes
+
+
 def stream_ptr(idx: int):
     """The library stream of device `idx` (cudaStream_t as an integer)."""
     s = _streams.get(idx)

@@ -668,6 +668,25 @@ def from_numpy(a: np.ndarray) -> Tensor:
                   _contig_strides(a.shape), dt, _CPU)
 
 
+def from_device_memory(ptr: int, shape, dtype, *, strides=None, device=0, owner=None) -> Tensor:
+    """A tensor over device memory of another library (`ptr`: its address, `strides` in elements,
+    row-major when omitted; `owner` is kept alive as long as the tensor's views).  Work on it runs
+    on this package's stream: wait for what other streams still do with the memory before the
+    first call, and synchronise before others read a result."""
+    dt = to_dtype(dtype)
+    shape = tuple(int(s) for s in shape)
+    strides = _contig_strides(shape) if strides is None else tuple(int(s) for s in strides)
+    if len(strides) != len(shape) or any(s < 0 for s in strides) or any(s < 0 for s in shape):
+        raise ValueError("from_device_memory: strides and shape have to be as many and not negative")
+    if ptr % dt.itemsize or (ptr == 0 and math.prod(shape)):
+        raise ValueError(f"from_device_memory: address {ptr:#x} for {dt.name}")
+    idx = int(getattr(device, "index", device) or 0)
+    _ensure_device(idx)
+    last = sum((n - 1) * s for n, s in zip(shape, strides)) if math.prod(shape) else -1
+    return Tensor(_rt.ExternalBuffer(ptr, (last + 1) * dt.itemsize, idx, owner), 0, shape, strides, dt,
+                  globals()["device"]("cuda", idx))
+
+
 def tensor(data, dtype=None, device=None, requires_grad=False):
     if isinstance(data, Tensor):
         t = data
