@@ -15,7 +15,7 @@ namespace mt {
 constexpr int kRowTile = 4;    // rows per CTA of attn_rows_kernel
 constexpr int kRowBlock = 16;  // keys per step of a warp
 
-enum { KV_ALIGNED = 0, KV_STRIDED = 1, KV_PAGED4 = 2 };
+enum { KV_ALIGNED = 0, KV_STRIDED = 1 };
 
 // One CTA (4 warps) = kRowTile rows of one (batch entry, key head) and one share of their keys.
 // A group of 8 lanes works on one key: a lane holds 4 channels of every 32.
@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7, grp = lane >> 3;
   const int bk = blockIdx.y, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int r0 = blockIdx.z * kRowTile, nr = min(kRowTile, p.rows - r0);
-  const SeqPos sp = seq_pos(p, b, KIND == KV_PAGED4);
+  const SeqPos sp = seq_pos(p, b, false);
 
   for (int i = threadIdx.x; i < kRowTile * DP; i += 128) {
     const int r = i / DP, d = i % DP;
@@ -61,17 +61,10 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
 
   for (int i = i0 + warp; i < i1; i += 4) {
     const int k0 = bl.block(i) * kRowBlock;
-    int64_t page_row = 0;
-    bool here = true;
-    if (KIND == KV_PAGED4) {
-      const int page = p.table[b * p.table_stride + (k0 >> p.page_shift)];
-      here = page >= 0 && page < p.num_pages;
-      page_row = (((int64_t)(here ? page : 0) * p.Hkv + hk) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
-    }
 #pragma unroll 1
     for (int it = 0; it < kRowBlock / 4; ++it) {
       const int kk = it * 4 + grp, key = k0 + kk;
-      const bool live = here && key < sp.n;
+      const bool live = key < sp.n;
       auto load = [&](int which, float (&x)[DCH][4]) {
 #pragma unroll
         for (int c = 0; c < DCH; ++c) {
@@ -79,27 +72,18 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[c][j] = 0.f;
           if (!live || d >= p.D) continue;
-          if (KIND == KV_PAGED4) {
-            const int64_t row = page_row + kk;
-            const uint32_t w = p.words[which][row * (p.D / 8) + d / 8] >> ((d & 4) * 4);
-            const __half2 sz = p.scales[which][row * (p.D / 64) + d / 64];
+          const int64_t* s = which ? p.vs : p.ks;
+          const T* src = static_cast<const T*>(which ? p.v : p.k) + b * s[0] + hk * s[1] + key * s[2];
+          if (KIND == KV_ALIGNED) {
+            alignas(16) T raw[4];
+            if (sizeof(T) == 4) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + d);
+            else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[c][j] = to_f32<T>(raw[j]);
+          } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              x[c][j] = fmaf((float)((w >> (4 * j)) & 15u), __low2float(sz), __high2float(sz));
-          } else {
-            const int64_t* s = which ? p.vs : p.ks;
-            const T* src = static_cast<const T*>(which ? p.v : p.k) + b * s[0] + hk * s[1] + key * s[2];
-            if (KIND == KV_ALIGNED) {
-              alignas(16) T raw[4];
-              if (sizeof(T) == 4) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + d);
-              else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src + d);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[c][j] = to_f32<T>(raw[j]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (d + j < p.D) x[c][j] = to_f32<T>(src[(d + j) * s[3]]);
-            }
+              if (d + j < p.D) x[c][j] = to_f32<T>(src[(d + j) * s[3]]);
           }
         }
       };
@@ -237,6 +221,26 @@ static int rows_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk
   return choose_splits(B * Hkv * tiles, span_keys(Sk, Sq, causal, window, sinks));
 }
 
+// Rows of head dim channels are whole 16-byte vectors of a 16-bit type.
+static bool aligned16(const void* base, const int64_t* s, int64_t D) {
+  return s[3] == 1 && D % 8 == 0 && (uintptr_t)base % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+}
+
+static bool takes_split(const mt_window_attention_desc& d) {
+  return d.dtype != MT_F32 && aligned16(d.k, d.k_strides, d.D) && aligned16(d.v, d.v_strides, d.D);
+}
+
+static int window_splits(const mt_window_attention_desc& d) {
+  if (takes_split(d))
+    return split_count(d.B * d.Hkv, d.Sq * (d.H / d.Hkv), span_keys(d.Sk, d.Sq, d.causal, d.window, d.sinks));
+  return rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks);
+}
+
+static int cache_splits(const mt_kv_cache4_attention_desc& d) {
+  return split_count(d.B * d.cache.Hkv, d.Sq * (d.H / d.cache.Hkv),
+                     span_keys(d.max_pages * d.cache.page_size, d.Sq, 1, d.window, d.sinks));
+}
+
 static void bind_workspace(AttnParams& p, void* ws) {
   const size_t rows = (size_t)p.B * p.Hkv * p.rows;
   p.part_ml = static_cast<float2*>(ws);
@@ -248,6 +252,10 @@ static int join_launch(const AttnParams& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
   attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p);
   return check_launch("attention_join");
+}
+
+static int join(const AttnParams& p, int dtype, cudaStream_t st) {
+  return dtype == MT_F16 ? join_launch<__half>(p, st) : join_launch<__nv_bfloat16>(p, st);
 }
 
 template <typename T, int KIND>
@@ -292,7 +300,7 @@ static int validate_window(const mt_window_attention_desc& d) {
 
 size_t window_attention_workspace(const mt_window_attention_desc& d) {
   if (validate_window(d) || d.B == 0 || d.Sq == 0) return 0;
-  return part_bytes(rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks), d.B * d.H * d.Sq, d.D);
+  return part_bytes(window_splits(d), d.B * d.H * d.Sq, d.D);
 }
 
 // 4 channels are one aligned vector
@@ -323,10 +331,14 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
   for (int i = 0; i < 4; ++i) {
     p.qs[i] = d.q_strides[i]; p.ks[i] = d.k_strides[i]; p.vs[i] = d.v_strides[i]; p.os[i] = d.o_strides[i];
   }
-  p.splits = rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks);
+  p.splits = window_splits(d);
   if (ws_bytes < window_attention_workspace(d) || (p.splits > 1 && !ws))
     return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
   bind_workspace(p, ws);
+  if (takes_split(d)) {
+    rc = run_split_attention(p, d.dtype, false, st);
+    return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
+  }
   switch (d.dtype) {
     case MT_F32: return window_dispatch<float>(d, p, st);
     case MT_BF16: return window_dispatch<__nv_bfloat16>(d, p, st);
@@ -350,8 +362,7 @@ static int validate_cache_attention(const mt_kv_cache4_attention_desc& d) {
 
 size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d) {
   if (validate_cache_attention(d) || d.B == 0 || d.Sq == 0) return 0;
-  return part_bytes(rows_splits(d.B, d.H, d.cache.Hkv, d.Sq, d.max_pages * d.cache.page_size, 1, d.window, d.sinks),
-                    d.B * d.H * d.Sq, d.cache.D);
+  return part_bytes(cache_splits(d), d.B * d.H * d.Sq, d.cache.D);
 }
 
 int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -376,12 +387,12 @@ int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size
   p.table = d.block_table; p.table_stride = d.table_stride;
   p.num_pages = (int)d.cache.num_pages;
   p.page_shift = __builtin_ctzll((unsigned long long)d.cache.page_size);
-  p.splits = rows_splits(d.B, d.H, d.cache.Hkv, d.Sq, p.Sk, 1, d.window, d.sinks);
+  p.splits = cache_splits(d);
   if (ws_bytes < kv_cache4_attention_workspace(d) || (p.splits > 1 && !ws))
     return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
   bind_workspace(p, ws);
-  if (d.dtype == MT_BF16) return rows_launch<__nv_bfloat16, KV_PAGED4>(p, st);
-  return rows_launch<__half, KV_PAGED4>(p, st);
+  rc = run_split_attention(p, d.dtype, true, st);
+  return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
 }
 
 }  // namespace mt

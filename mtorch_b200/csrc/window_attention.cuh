@@ -29,6 +29,7 @@ struct AttnParams {
   int num_pages, page_shift;
   // split keys: partial results in the workspace
   int splits;
+  int target;       // CTAs that the work is cut into (attn_split_kernel)
   float2* part_ml;  // [split][B * Hkv * rows] (maximum in base 2, sum)
   float* part_o;    // [split][B * Hkv * rows][D], not divided by the sum
 };
@@ -75,5 +76,9 @@ __device__ __forceinline__ BlockList block_list(const AttnParams& p, const SeqPo
   l.count = l.first + max(0, last - l.from + 1);
   return l;
 }
+
+// window_attention_split.cu: few query rows over 16-bit keys (16-byte aligned rows) or the 4-bit cache
+int split_count(int64_t bk, int64_t rows, int64_t keys);
+int run_split_attention(AttnParams& p, int dtype, bool paged, cudaStream_t st);
 
 }  // namespace mt
