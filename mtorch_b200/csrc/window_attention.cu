@@ -164,33 +164,81 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
   }
 }
 
-// One warp joins the shares of one row.
+// One CTA joins the shares of one row: groups of threads take shares in turn, a thread holds 4 channels (or
+// single ones where D is no multiple of 4), so that all the reads of a row are in flight at once.
+constexpr int kJoinThreads = 256;
+constexpr int kMaxSplits = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParams p) {
+  __shared__ float w[kMaxSplits];
+  __shared__ float red[kJoinThreads * 4];
+  __shared__ float s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
+  // launched while the kernel before it still runs (see join_launch): wait for its results
+  cudaGridDependencySynchronize();
   const int64_t total = (int64_t)p.B * p.Hkv * p.rows;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= total) return;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float2 ml[kMaxSplits / kJoinThreads];
   float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[s * total + row].x);
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / kJoinThreads; ++i) {
+    const int s = tid + i * kJoinThreads;
+    ml[i] = s < p.splits ? p.part_ml[s * total + row] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
   top = warp_max(top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, s_top[i]);
   float ls = 0.f;
-  for (int s = lane; s < p.splits; s += 32) {
-    const float2 ml = p.part_ml[s * total + row];
-    if (ml.x != -INFINITY) ls = fmaf(ml.y, exp2f(ml.x - top), ls);
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / kJoinThreads; ++i) {
+    const int s = tid + i * kJoinThreads;
+    const float f = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - top);
+    if (s < p.splits) w[s] = f;
+    ls = fmaf(ml[i].y, f, ls);
   }
   ls = warp_sum(ls);
+  if (lane == 0) s_sum[warp] = ls;
+  __syncthreads();
+  ls = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) ls += s_sum[i];
+
+  const bool vec = p.D % 4 == 0;
+  const int n = vec ? p.D / 4 : p.D, groups = max(1, kJoinThreads / n);
+  const int g = tid / n, c = tid % n;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g < groups) {
+#pragma unroll 4
+    for (int s = g; s < p.splits; s += groups) {
+      const float f = w[s];
+      if (f == 0.f) continue;  // an empty share wrote no o
+      const float* src = p.part_o + (s * total + row) * p.D;
+      if (vec) {
+        const float4 v = reinterpret_cast<const float4*>(src)[c];
+        x.x = fmaf(v.x, f, x.x);
+        x.y = fmaf(v.y, f, x.y);
+        x.z = fmaf(v.z, f, x.z);
+        x.w = fmaf(v.w, f, x.w);
+      } else {
+        x.x = fmaf(src[c], f, x.x);
+      }
+    }
+  }
+  reinterpret_cast<float4*>(red)[tid] = x;
+  __syncthreads();
   const int64_t bk = row / p.rows;
   const int r = (int)(row - bk * p.rows);
   const int b = (int)(bk / p.Hkv), hk = (int)(bk % p.Hkv);
   T* dst = static_cast<T*>(p.o) + b * p.os[0] + (hk * p.g + r % p.g) * p.os[1] + (r / p.g) * p.os[2];
-  for (int d = lane; d < p.D; d += 32) {
-    float x = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float ms = p.part_ml[s * total + row].x;
-      if (ms != -INFINITY) x = fmaf(p.part_o[(s * total + row) * p.D + d], exp2f(ms - top), x);
-    }
-    dst[d * p.os[3]] = from_f32<T>(ls > 0.f ? x / ls : 0.f);
+  for (int d = tid; d < p.D; d += kJoinThreads) {
+    const int at = vec ? d : d * 4, step = n * 4;
+    float y = 0.f;
+    for (int i = 0; i < groups; ++i) y += red[i * step + at];
+    dst[d * p.os[3]] = from_f32<T>(ls > 0.f ? y / ls : 0.f);
   }
 }
 
@@ -207,7 +255,7 @@ static int64_t span_keys(int64_t Sk, int64_t Sq, int causal, int64_t window, int
 static int choose_splits(int64_t ctas, int64_t keys) {
   const int64_t want = (4LL * num_sms() + ctas - 1) / ctas;
   const int64_t most = std::max<int64_t>(1, keys / (8 * kRowBlock));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 512));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), kMaxSplits));
 }
 
 static size_t part_bytes(int splits, int64_t rows, int64_t D) {
@@ -250,8 +298,19 @@ static void bind_workspace(AttnParams& p, void* ws) {
 template <typename T>
 static int join_launch(const AttnParams& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
-  attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p);
-  return check_launch("attention_join");
+  if (rows > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "window_attention: too many rows");
+  // programmatic launch: the CTAs come up while the last shares are computed, which hides the launch
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  int rc = cuda_check(cudaLaunchKernelEx(&cfg, attn_join_kernel<T>, p), "attention_join");
+  return rc ? rc : check_launch("attention_join");
 }
 
 static int join(const AttnParams& p, int dtype, cudaStream_t st) {
@@ -336,6 +395,7 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
     return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
   bind_workspace(p, ws);
   if (takes_split(d)) {
+    p.q_vec = aligned16(d.q, d.q_strides, d.D);
     rc = run_split_attention(p, d.dtype, false, st);
     return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
   }
@@ -391,6 +451,7 @@ int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size
   if (ws_bytes < kv_cache4_attention_workspace(d) || (p.splits > 1 && !ws))
     return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
   bind_workspace(p, ws);
+  p.q_vec = aligned16(d.q, d.q_strides, d.cache.D);
   rc = run_split_attention(p, d.dtype, true, st);
   return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
 }

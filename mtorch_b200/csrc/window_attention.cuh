@@ -29,6 +29,7 @@ struct AttnParams {
   int num_pages, page_shift;
   // split keys: partial results in the workspace
   int splits;
+  int q_vec;        // 8 channels of q are one aligned 16-byte vector (attn_split_kernel)
   int target;       // CTAs that the work is cut into (attn_split_kernel)
   float2* part_ml;  // [split][B * Hkv * rows] (maximum in base 2, sum)
   float* part_o;    // [split][B * Hkv * rows][D], not divided by the sum

@@ -8,13 +8,15 @@
 // bytes of codes) at a time, with no shared memory between: the k order of a product is free, and the
 // codes are unpacked into fragments with one shift and one logic instruction per pair.
 //
-// Codes as operands: bf16 takes 0x4300 | c = 128 + c, exact; f16 takes the code's bits as they are, a
-// subnormal c * 2^-24, exact too.  With value = zero + scale c,
-//   q.k = scale (q.(128 + c)) + (zero - 128 scale) sum(q)   per 64 channels,
-// on fp32 sums that start anew for each 16 keys.  V's codes run over thousands of keys into one
-// sum, which an offset of 128 would bias (the tensor core truncates), so they are centred exactly:
-//   o = sum p scale (c - 8) + sum p (zero + 8 scale),
-// with p scale rounded to bf16 (for f16 queries too: p scale spans more than f16's exponents).
+// Codes as operands: the 4 bits of a code at the low end of a 16-bit lane ARE the number c * 2^-133 in
+// bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly; at bits 4..7 they are 16 times that.  One
+// AND makes two operands, one shift serves half a word.  bf16 queries are scaled by 2^64 (exact) to keep
+// the products far from fp32's own subnormals, their channels at bits 4..7 by 2^60.  With value = zero + scale c:
+//   q.k = scale (q.c) + zero sum(q)  per 64 channels,
+//   o   = sum (p scale) c + sum p zero,
+// with p scale rounded to bf16 (for f16 queries too: p scale spans more than f16's exponents).  That
+// rounding meets c - 8 rather than c, because what is added for zero is p (zero + 8 scale) - 8 round(p scale):
+// the codes of a key centre around 8, and the error of a rounded weight is halved.
 //
 // The running maximum is raised only when a score passes it by more than 2^8 ("lazy"): then the warp
 // reduces the maximum and rescales; otherwise a block of 16 keys costs one vote.
@@ -46,54 +48,106 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same on accumulators of zero
+template <bool F16>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // transpose of an 8 x 8 matrix of 16-bit elements spread over the warp (row lane / 4, columns 2 (lane % 4) ..)
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// two codes at bits 4i and 16 + 4i as 128 + c (bf16) or c * 2^-24 (f16)
-template <bool F16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
-  return ((w >> (4 * i)) & 0x000f000fu) | (F16 ? 0u : 0x43004300u);
+// operands of codes i and i + 4 of a word: c * u, or 16 c * u for odd i (u = 2^-133 in bf16, 2^-24 in f16)
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int i) {
+  return (i & 2 ? w8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
 }
-// the same two codes minus 8, exact in bf16
-__device__ __forceinline__ uint32_t code_pair_centred(uint32_t w, int i) {
-  const uint32_t x = code_pair<false>(w, i);
-  __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&x);
-  v = __hsub2(v, __nv_bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));  // 136
-  return *reinterpret_cast<const uint32_t*>(&v);
+constexpr float kPow64 = 18446744073709551616.f;          // 2^64
+constexpr float kPow69 = 32.f * kPow64;                    // 2^69 = 2^133 / 2^64
+
+// 16 bytes to shared memory, zeros when !live
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// 16 bytes to shared memory where `on`
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(dst),
+               "l"(src), "r"((int)on)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ uint4 ldg16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
+// A warp's ring of steps (KB blocks of 16 keys) in shared memory, filled by the warp's own cp.async (no barrier
+// between warps).  The 16-byte chunks are placed so that the fragment reads meet no bank twice:
+//   16-bit rows (8 DC chunks): chunk ch of K row r at ch ^ kswz(r), of V row r at ch ^ (r & 7);
+//   rows of codes (2 DC chunks, DC halves of 32 bytes): a block's V rows in the order 0 2 4 .. 1 3 5 .., then half
+//   c of the row at place r at c ^ (r / 2) for DC = 2, c ^ r for DC = 4.
+template <bool PAGED, int DC, int KB>
+struct SplitRing {
+  static constexpr int ROW = PAGED ? 32 * DC : 128 * DC;         // bytes of a row of K or V
+  static constexpr int SCALES = PAGED ? KB * 16 * 4 * DC : 0;    // bytes of a step's scales of K or V
+  static constexpr int RUN = KB * 16 * ROW;                      // bytes of a step's K or V
+  static constexpr int STAGE = 2 * (RUN + SCALES);
+  static constexpr int STAGES = PAGED && KB == 1 ? 4 : 3;
+  static constexpr int BYTES = STAGE * STAGES;                   // a warp's
+  static constexpr int V = RUN, KS = 2 * RUN, VS = KS + SCALES;  // offsets in a stage; K at 0
+  static_assert(!PAGED || 4 * DC * KB <= 16, "a step's scales are one instruction of the warp");
+  static __device__ __forceinline__ int kswz(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+  static __device__ __forceinline__ int half(int c, int r) { return DC == 2 ? c ^ ((r >> 1) & 1) : DC == 4 ? c ^ (r & 3) : c; }
+  static __device__ __forceinline__ int vplace(int r) { return (r & 16) | ((r & 15) >> 1) | ((r & 1) << 3); }
+};
 
-// One CTA: kSplitWarps warps over one chunk of the key blocks of (b, hk) for 8 * NT query rows.
-// DC: blocks of 64 channels.  In a lane, n = lane / 4 and t = lane % 4.
-template <bool F16, bool PAGED, int DC, int NT>
-__global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const AttnParams p) {
+// One CTA: kSplitWarps warps over one chunk of the steps (KB blocks of 16 keys, of one page) of (b, hk) for
+// 8 * NT query rows.  DC: blocks of 64 channels.  In a lane, n = lane / 4 and t = lane % 4.
+template <bool F16, bool PAGED, int DC, int NT, int KB>
+__global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 2) : 1) attn_split_kernel(const AttnParams p) {
   using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
   constexpr int ROWS = 8 * NT;
   constexpr int DP = 64 * DC;
   constexpr bool PF16 = F16 && !PAGED;  // type of P and V's operands
-  __shared__ float so[ROWS][DP + 4];
+  using Ring = SplitRing<PAGED, DC, KB>;
+  constexpr int STEP = 16 * KB;  // keys
+  static_assert(ROWS * (DP + 4) * 4 <= Ring::BYTES, "the ring holds a warp's result at the end");
+  extern __shared__ __align__(16) uint8_t split_smem[];
   __shared__ float2 sml[kSplitWarps][ROWS];
+  __shared__ RowKeys srk[ROWS];
+  __shared__ float sinv[ROWS];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
   const int bk = blockIdx.y, b = bk / p.Hkv, hk = bk % p.Hkv;
   const int r0 = blockIdx.z * ROWS, nr = min(ROWS, p.rows - r0);
   const SeqPos sp = seq_pos(p, b, PAGED);
-  const int pmin = sp.start + r0 / p.g, pmax = sp.start + (r0 + nr - 1) / p.g;
-  const BlockList bl = block_list<16>(p, sp, pmin, pmax);
+  const int q0 = r0 / p.g, q1 = (r0 + nr - 1) / p.g;  // queries of the rows
+  const int pmin = sp.start + q0, pmax = sp.start + q1;
+  const BlockList bl = block_list<STEP>(p, sp, pmin, pmax);
 
-  // chunk: the same for every CTA of the grid, so that sequences of different lengths fill it evenly
-  float total = 0.f;  // blocks of the whole batch; a guide only, but the same in every CTA
-  for (int i = lane; i < p.B; i += 32) {
-    const SeqPos s = seq_pos(p, i, PAGED);
-    total += (float)block_list<16>(p, s, s.start + r0 / p.g, s.start + (r0 + nr - 1) / p.g).count;
+  // chunk: about the same for every CTA of the grid, so that sequences of different lengths fill it evenly
+  int per = bl.count;
+  if (gridDim.x > 1) {
+    float total = 0.f;  // steps of the whole batch; a guide only, but the same in every CTA
+    for (int i = lane; i < p.B; i += 32) {
+      const SeqPos s = seq_pos(p, i, PAGED);
+      total += (float)block_list<STEP>(p, s, s.start + q0, s.start + q1).count;
+    }
+    total = warp_sum(total) * (float)(p.Hkv * gridDim.z) / (float)p.target;
+    per = max(kMinChunk / KB, (int)fminf(ceilf(total), (float)bl.count));
+    const int chunks = min((bl.count + per - 1) / per, (int)gridDim.x);
+    per = chunks > 0 ? (bl.count + chunks - 1) / chunks : 1;  // of one length within the sequence
   }
-  total = warp_sum(total) * (float)(p.Hkv * gridDim.z) / (float)p.target;
-  int per = max(kMinChunk, (int)fminf(ceilf(total), (float)bl.count));
-  per = max(per, (bl.count + (int)gridDim.x - 1) / (int)gridDim.x);
   const int i0 = (int)min((int64_t)blockIdx.x * per, (int64_t)bl.count), i1 = min(bl.count, i0 + per);
   const int64_t out_row = ((int64_t)blockIdx.x * p.B * p.Hkv + bk) * p.rows + r0;
   if (i0 >= i1 && gridDim.x > 1) {
@@ -113,18 +167,31 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
 #pragma unroll
     for (int c = 0; c < 2 * DC; ++c) {
       const int base = PAGED ? (c >> 1) * 64 + t * 16 + (c & 1) * 8 : c * 32 + t * 8;
-      T v[8];
+      float v[8];
+      uint16_t u[8];
+      alignas(16) T raw[8];
+      if (p.q_vec) {  // (D is a multiple of 8)
+        *reinterpret_cast<uint4*>(raw) = live && base < p.D ? __ldg(reinterpret_cast<const uint4*>(src + base)) : make_uint4(0, 0, 0, 0);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = live && base + j < p.D ? src[(base + j) * p.qs[3]] : from_f32<T>(0.f);
-      const uint16_t* u = reinterpret_cast<const uint16_t*>(v);
+        for (int j = 0; j < 8; ++j) raw[j] = live && base + j < p.D ? src[(base + j) * p.qs[3]] : from_f32<T>(0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = to_f32<T>(raw[j]);
+        if (p.scale_log2 < 0.f) v[j] = -v[j];  // the maximum is taken of unscaled scores
+        const float f = !PAGED ? 1.f : (F16 ? 1.f : kPow64) * (j & 1 ? 0.0625f : 1.f);
+        const T h = from_f32<T>(v[j] * f);
+        u[j] = *reinterpret_cast<const uint16_t*>(&h);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         qf[x][c][j] = PAGED ? (u[j] | (uint32_t)u[j + 4] << 16) : (u[2 * j] | (uint32_t)u[2 * j + 1] << 16);
       if (PAGED) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += to_f32<T>(v[j]);
+        for (int j = 0; j < 8; ++j) s += v[j];
+        s *= F16 ? 1.f / 16777216.f : 1.f / kPow69;  // the unit of q.c below
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
@@ -133,20 +200,23 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
       }
     }
   }
-  // keys that the rows of this lane's columns (2t, 2t + 1) see; keys that all rows see, that any row sees
-  RowKeys rk[NT][2];
-#pragma unroll
-  for (int x = 0; x < NT; ++x)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) rk[x][j] = row_keys(p, sp, sp.start + (r0 + min(8 * x + 2 * t + j, nr - 1)) / p.g);
+  // keys that each row sees; keys that all rows see (ra.hi, rz.lo, ra.sk), that any row sees (ra.lo, rz.hi, rz.sk)
+  if (threadIdx.x < ROWS) srk[threadIdx.x] = row_keys(p, sp, sp.start + (r0 + min((int)threadIdx.x, nr - 1)) / p.g);
   const RowKeys ra = row_keys(p, sp, pmin), rz = row_keys(p, sp, pmax);
+  __syncthreads();
 
-  float m[NT][2], l[NT][2], cor[NT][DC][2], o[DC][4][NT][4];
+  // scores, their running maximum m and the bound `thr` past which it is raised are in units of
+  // 1 / score_scale (base 2); p = 2^(score - m + kShift)
+  constexpr float kShift = PAGED ? 64.f : 0.f;
+  const float score_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * (!PAGED ? 1.f : F16 ? 16777216.f : kPow69);
+  float m[NT][2], thr[NT][2], negm[NT][2], l[NT][2], cor[NT][DC][2], o[DC][4][NT][4];
+  float psum[PAGED ? DC : 1][NT][4];  // sums of the rounded weights, as a product with ones
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      m[x][j] = -INFINITY;
+      m[x][j] = thr[x][j] = -INFINITY;
+      negm[x][j] = kShift;
       l[x][j] = 0.f;
 #pragma unroll
       for (int c = 0; c < DC; ++c) cor[x][c][j] = 0.f;
@@ -154,152 +224,212 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
 #pragma unroll
   for (int c = 0; c < DC; ++c)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[c][j][x][e] = 0.f;
-
-  // ---- loads: K and V of one block of 16 keys into registers ----
-  uint4 kd[PAGED ? 1 : 2 * DC][2];
-  uint2 kq[PAGED ? DC : 1][2];
-  uint4 vd[PAGED ? 1 : DC][4];
-  uint32_t vq[PAGED ? DC : 1][4];
-  __half2 ksc[PAGED ? DC : 1][2], vsc[PAGED ? DC : 1][2];
-  const T* kbase = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[1];
-  const T* vbase = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[1];
-
-  auto page_of = [&](int i) -> int {
-    if (!PAGED || i >= i1) return -1;
-    return __ldg(p.table + b * p.table_stride + ((bl.block(i) * 16) >> p.page_shift));
-  };
-  // row of the cache's arrays where block i starts (page -1 where the page does not exist)
-  auto cache_row = [&](int i, int page) -> int64_t {
-    return (((int64_t)page * p.Hkv + hk) << p.page_shift) + ((bl.block(i) * 16) & ((1 << p.page_shift) - 1));
-  };
-  auto load_k = [&](int i, int page) {
-    if (PAGED) {
-      if (i >= i1 || page < 0 || page >= p.num_pages) return;
-      const int64_t row = cache_row(i, page);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t rr = row + n + 8 * h;
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          kq[c][h] = __ldg(reinterpret_cast<const uint2*>(p.words[0] + rr * (DP / 8) + c * 8 + t * 2));
-          ksc[c][h] = __ldg(p.scales[0] + rr * DC + c);
-        }
-      }
-    } else {
-      const int k0 = bl.block(i) * 16;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = k0 + n + 8 * h;
-        const T* src = kbase + (int64_t)key * p.ks[2] + t * 8;
-#pragma unroll
-        for (int c = 0; c < 2 * DC; ++c)
-          kd[c][h] = (i < i1 && key < sp.n && c * 32 + t * 8 < p.D) ? ldg16(src + c * 32) : make_uint4(0, 0, 0, 0);
-      }
-    }
-  };
-  auto load_v = [&](int i, int page) {
-    if (PAGED) {
-      if (i >= i1 || page < 0 || page >= p.num_pages) return;
-      const int64_t row = cache_row(i, page);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t rr = row + 2 * t + (e & 1) + (e >> 1) * 8;
-#pragma unroll
-        for (int c = 0; c < DC; ++c) vq[c][e] = __ldg(p.words[1] + rr * (DP / 8) + c * 8 + n);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < DC; ++c) vsc[c][h] = __ldg(p.scales[1] + (row + n + 8 * h) * DC + c);
-    } else {
-      const int k0 = bl.block(i) * 16;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 2 * t + (e & 1) + (e >> 1) * 8;
-        // a key that no row sees counts as zeros, whatever stands there
-        const bool live = i < i1 && key < sp.n && ((key >= ra.lo && key <= rz.hi) || key < rz.sk);
-        const T* src = vbase + (int64_t)key * p.vs[2] + n * 8;
-#pragma unroll
-        for (int c = 0; c < DC; ++c)
-          vd[c][e] = (live && c * 64 + n * 8 < p.D) ? ldg16(src + c * 64) : make_uint4(0, 0, 0, 0);
-      }
-    }
-  };
-
-  int i = i0 + warp;
-  int page = page_of(i), page_next = page_of(i + kSplitWarps);
-  load_k(i, page);
-  load_v(i, page);
-  for (; i < i1; i += kSplitWarps) {
-    const int k0 = bl.block(i) * 16;
-    // ---- S^T = K Q^T: sc[.][0,1] key n, sc[.][2,3] key n + 8; columns 2t, 2t + 1 ----
-    float sc[NT][4];
-#pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[x][e] = 0.f;
-    if (PAGED) {
+      for (int e = 0; e < 4; ++e) {
 #pragma unroll
-      for (int c = 0; c < DC; ++c) {
-        float acc[NT][4];
+        for (int j = 0; j < 4; ++j) o[c][j][x][e] = 0.f;
+        psum[PAGED ? c : 0][x][e] = 0.f;
+      }
+
+  // ---- loads: steps of keys into this warp's ring ----
+  uint8_t* ring = split_smem + warp * Ring::BYTES;
+  const uint32_t ring_u32 = smem_u32(ring);
+  const int64_t es = sizeof(T);
+  // sources: paged, this lane's chunk of a step's words and scales; dense, the head's first row
+  constexpr int CH = PAGED ? 2 * DC : 8 * DC;  // chunks of a row
+  const uint8_t *ksrc, *vsrc, *ssrc = nullptr;
+  if (PAGED) {
+    const uint64_t head = ((uint64_t)hk << p.page_shift);  // rows
+    ksrc = reinterpret_cast<const uint8_t*>(p.words[0]) + head * Ring::ROW + lane * 16;
+    vsrc = reinterpret_cast<const uint8_t*>(p.words[1]) + head * Ring::ROW + lane * 16;
+    ssrc = reinterpret_cast<const uint8_t*>(p.scales[lane >> 4]) + head * (4 * DC) + (lane & 15) * 16;
+  } else {
+    ksrc = static_cast<const uint8_t*>(p.k) + (b * p.ks[0] + hk * p.ks[1]) * es;
+    vsrc = static_cast<const uint8_t*>(p.v) + (b * p.vs[0] + hk * p.vs[1]) * es;
+  }
+  // where chunk j * 32 + lane goes (the offsets of j > 0 are constants for DC <= 2)
+  auto kdst = [&](int j) {
+    const int r = (j * 32 + lane) / CH, ch = (j * 32 + lane) % CH;
+    return PAGED ? r * Ring::ROW + Ring::half(ch >> 1, r) * 32 + (ch & 1) * 16 : r * Ring::ROW + (ch ^ Ring::kswz(r)) * 16;
+  };
+  auto vdst = [&](int j) {
+    const int r = (j * 32 + lane) / CH, ch = (j * 32 + lane) % CH;
+    const int v = Ring::vplace(r);
+    return PAGED ? v * Ring::ROW + Ring::half(ch >> 1, v) * 32 + (ch & 1) * 16 : r * Ring::ROW + (ch ^ (r & 7)) * 16;
+  };
+  const uint32_t kdst0 = kdst(0), vdst0 = vdst(0);
+  const uint32_t sdst = (lane >> 4 ? Ring::VS : Ring::KS) + (lane & 15) * 16;
+  const int32_t* table = p.table + b * p.table_stride;
+  // row (in units of 16) of step i in the cache's arrays (of head 0), kNoRow where its page does not exist; steps
+  // past the chunk look at its last one
+  constexpr uint32_t kNoRow = 0xffffffffu;
+  const uint32_t page_blocks = (uint32_t)p.Hkv << (p.page_shift - 4);
+  auto cache_row = [&](int i) -> uint32_t {
+    const int k0 = bl.block(min(i, i1 - 1)) * STEP;
+    const int page = __ldg(table + (k0 >> p.page_shift));
+    const uint32_t row = (uint32_t)page * page_blocks + ((k0 & ((1 << p.page_shift) - 1)) >> 4);
+    return i < i1 && (uint32_t)page < (uint32_t)p.num_pages ? row : kNoRow;
+  };
+  // brings step i to `stage`
+  auto load = [&](int i, uint32_t row, int stage) {
+    const uint32_t dst = ring_u32 + stage * Ring::STAGE;
+    if (PAGED) {
+      const bool on = row != kNoRow;
+      const uint8_t* ks = ksrc + (uint64_t)row * (16 * Ring::ROW);
+      const uint8_t* vs = vsrc + (uint64_t)row * (16 * Ring::ROW);
+#pragma unroll
+      for (int j = 0; j < KB * DC; ++j) {
+        // 32 chunks are 16 / DC rows: rows + 8 (DC = 2) or + 16 keep the swizzle, V's places move by 4 and 16
+        const uint32_t ko = DC <= 2 ? kdst0 + j * 512 : kdst(j);
+        const uint32_t vo = DC == 1 ? vdst0 + j * 512 : DC == 2 ? vdst0 + ((j & 1) * 4 + (j >> 1) * 16) * Ring::ROW : vdst(j);
+        cp_async16_if(dst + ko, ks + j * 512, on);
+        cp_async16_if(dst + Ring::V + vo, vs + j * 512, on);
+      }
+      cp_async16_if(dst + sdst, ssrc + (uint64_t)row * (16 * 4 * DC), on && (lane & 15) < 4 * DC * KB);
+    } else if (i < i1) {
+      const int k0 = bl.block(i) * STEP;
+      // channels past D are zeros; RPI rows an instruction where rows do not straddle instructions
+      if (32 % CH == 0 && k0 + STEP <= sp.n && (k0 + STEP - 1 <= rz.hi && (k0 >= ra.lo || k0 + STEP - 1 < rz.sk))) {
+        constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;
+        const int r = lane / CH, ch = lane % CH;
+        const uint8_t* ks = ksrc + ((k0 + r) * p.ks[2] + ch * 8) * es;
+        const uint8_t* vs = vsrc + ((k0 + r) * p.vs[2] + ch * 8) * es;
+        const int64_t kstep = RPI * p.ks[2] * es, vstep = RPI * p.vs[2] * es;
+        const bool in = ch * 8 < p.D;
+#pragma unroll
+        for (int j = 0; j < STEP / RPI; ++j) {
+          cp_async16(dst + kdst(j), in ? ks : ksrc, in);
+          cp_async16(dst + Ring::V + vdst(j), in ? vs : vsrc, in);
+          ks += kstep;
+          vs += vstep;
+        }
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < STEP * CH / 32; ++j) {
+          const int r = (j * 32 + lane) / CH, ch = (j * 32 + lane) % CH;
+          const int key = k0 + r;
+          const bool in = key < sp.n && ch * 8 < p.D;
+          // a key that no row sees counts as zeros in V, whatever stands there
+          const bool seen = in && ((key >= ra.lo && key <= rz.hi) || key < rz.sk);
+          cp_async16(dst + kdst(j), in ? ksrc + (key * p.ks[2] + ch * 8) * es : ksrc, in);
+          cp_async16(dst + Ring::V + vdst(j), seen ? vsrc + (key * p.vs[2] + ch * 8) * es : vsrc, seen);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+
+  // this lane's fragments in a stage
+  int koff[DC], voff[DC];
+#pragma unroll
+  for (int c = 0; c < DC; ++c) {
+    koff[c] = n * Ring::ROW + Ring::half(c, n) * 32 + t * 8;              // rows n, n + 8
+    voff[c] = Ring::V + t * Ring::ROW + Ring::half(c, t) * 32 + n * 4;    // places t (+ 8, 4, 12): rows 2t, 2t + 1, 2t + 8, 2t + 9
+  }
+
+  int i = i0 + warp;
+  uint32_t row_next = kNoRow;   // of the next step to bring: looked up a step early
+  uint32_t missing_steps = 0;   // bit s: step i + s W has no page
+  if (PAGED && i0 < i1) row_next = cache_row(i);
+#pragma unroll
+  for (int s = 0; s < Ring::STAGES - 1; ++s) {
+    load(i + s * kSplitWarps, row_next, s);
+    if (PAGED && i0 < i1) {
+      missing_steps |= (uint32_t)(row_next == kNoRow) << s;
+      row_next = cache_row(i + (s + 1) * kSplitWarps);
+    }
+  }
+  int stage = 0;
+  for (; i < i1; i += kSplitWarps) {
+    const int k0 = bl.block(i) * STEP;
+    cp_async_wait<Ring::STAGES - 2>();
+    __syncwarp();
+    const uint8_t* st = ring + stage * Ring::STAGE;
+    // ---- S^T = K Q^T: sc[.][.][0,1] key n of a block, [2,3] key n + 8; columns 2t, 2t + 1 ----
+    float sc[KB][NT][4];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      if (PAGED) {
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          float acc[NT][4];
+          uint2 kq[2];
+          float2 ksc[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kq[h] = *reinterpret_cast<const uint2*>(st + koff[c] + (kb * 16 + 8 * h) * Ring::ROW);
+            ksc[h] = __half22float2(*reinterpret_cast<const __half2*>(st + n * (4 * DC) + Ring::KS + ((kb * 16 + 8 * h) * DC + c) * 4));
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t w0 = u ? kq[0].y : kq[0].x, w1 = u ? kq[1].y : kq[1].x;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t a[4] = {code_pair(w0, w0 >> 8, 2 * e), code_pair(w1, w1 >> 8, 2 * e),
+                                     code_pair(w0, w0 >> 8, 2 * e + 1), code_pair(w1, w1 >> 8, 2 * e + 1)};
+#pragma unroll
+              for (int x = 0; x < NT; ++x) {
+                if (u + e == 0) mma16816_zero<F16>(acc[x], a, qf[x][2 * c + u][2 * e], qf[x][2 * c + u][2 * e + 1]);
+                else mma16816<F16>(acc[x], a, qf[x][2 * c + u][2 * e], qf[x][2 * c + u][2 * e + 1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                sc[kb][x][2 * h + j] =
+                    fmaf(ksc[h].y, qsum[x][c][j], c ? fmaf(ksc[h].x, acc[x][2 * h + j], sc[kb][x][2 * h + j])
+                                                    : ksc[h].x * acc[x][2 * h + j]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2 * DC; ++c) {
+          const uint8_t* r0p = st + (kb * 16 + n) * Ring::ROW;
+          const uint4 k0v = *reinterpret_cast<const uint4*>(r0p + (((c * 4 + t) ^ Ring::kswz(n)) * 16));
+          const uint4 k1v = *reinterpret_cast<const uint4*>(r0p + 8 * Ring::ROW + (((c * 4 + t) ^ Ring::kswz(n)) * 16));
+          const uint32_t a0[4] = {k0v.x, k1v.x, k0v.y, k1v.y}, a1[4] = {k0v.z, k1v.z, k0v.w, k1v.w};
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            if (c == 0) mma16816_zero<F16>(sc[kb][x], a0, qf[x][c][0], qf[x][c][1]);
+            else mma16816<F16>(sc[kb][x], a0, qf[x][c][0], qf[x][c][1]);
+            mma16816<F16>(sc[kb][x], a1, qf[x][c][2], qf[x][c][3]);
+          }
+        }
+      }
+    }
+
+    // ---- softmax ----
+    const bool missing = PAGED && (missing_steps & 1u);
+    const bool full = !missing && k0 + STEP - 1 <= ra.hi && (k0 >= rz.lo || k0 + STEP - 1 < ra.sk);
+    if (!full) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint32_t w0 = u ? kq[c][0].y : kq[c][0].x, w1 = u ? kq[c][1].y : kq[c][1].x;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const uint32_t a[4] = {code_pair<F16>(w0, 2 * s), code_pair<F16>(w1, 2 * s),
-                                   code_pair<F16>(w0, 2 * s + 1), code_pair<F16>(w1, 2 * s + 1)};
-#pragma unroll
-            for (int x = 0; x < NT; ++x) mma16816<F16>(acc[x], a, qf[x][2 * c + u][2 * s], qf[x][2 * c + u][2 * s + 1]);
-          }
+          for (int e = 0; e < 4; ++e)
+            if (missing || !srk[8 * x + 2 * t + (e & 1)].sees(k0 + kb * 16 + n + 8 * (e >> 1))) sc[kb][x][e] = -INFINITY;
+      if (PAGED) {  // scales of slots that hold nothing may be NaN
+        for (int j = lane; j < STEP * DC; j += 32) {
+          const int key = k0 + j / DC;
+          if (missing || !((key >= ra.lo && key <= rz.hi) || key < rz.sk))
+            reinterpret_cast<uint32_t*>(ring + stage * Ring::STAGE + Ring::VS)[j] = 0u;
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float s = __low2float(ksc[c][h]), z = __high2float(ksc[c][h]);
-          const float f = F16 ? s * 16777216.f : s;
-          const float off = F16 ? z : fmaf(-128.f, s, z);
-#pragma unroll
-          for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              sc[x][2 * h + j] += fmaf(f, acc[x][2 * h + j], off * qsum[x][c][j]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 2 * DC; ++c) {
-        const uint32_t a0[4] = {kd[c][0].x, kd[c][1].x, kd[c][0].y, kd[c][1].y};
-        const uint32_t a1[4] = {kd[c][0].z, kd[c][1].z, kd[c][0].w, kd[c][1].w};
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          mma16816<F16>(sc[x], a0, qf[x][c][0], qf[x][c][1]);
-          mma16816<F16>(sc[x], a1, qf[x][c][2], qf[x][c][3]);
-        }
+        __syncwarp();
       }
     }
-    const bool missing = PAGED && (page < 0 || page >= p.num_pages);
-    load_k(i + kSplitWarps, page_next);
-
-    // ---- softmax ----
-    const bool full = !missing && k0 + 15 <= ra.hi && (k0 >= rz.lo || k0 + 15 < ra.sk);
     bool over = false;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float s = sc[x][e] * p.scale_log2;
-        if (!full && (missing || !rk[x][e & 1].sees(k0 + n + 8 * (e >> 1)))) s = -INFINITY;
-        sc[x][e] = s;
-        over |= s > m[x][e & 1] + kSplitLazy;
+      for (int j = 0; j < 2; ++j) {
+        float top = fmaxf(sc[0][x][j], sc[0][x][2 + j]);
+        if (KB == 2) top = fmaxf(top, fmaxf(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
+        over |= top > thr[x][j];
       }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -307,16 +437,22 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
         float corr[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float mx = fmaxf(sc[x][j], sc[x][2 + j]);
+          float mx = fmaxf(sc[0][x][j], sc[0][x][2 + j]);
+          if (KB == 2) mx = fmaxf(mx, fmaxf(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           mx = fmaxf(mx, m[x][j]);
-          corr[j] = m[x][j] == -INFINITY ? 0.f : ex2f(m[x][j] - mx);
+          corr[j] = m[x][j] == -INFINITY ? 0.f : ex2f((m[x][j] - mx) * score_scale);
           m[x][j] = mx;
+          thr[x][j] = mx + kSplitLazy / score_scale;
+          negm[x][j] = mx == -INFINITY ? kShift : fmaf(-mx, score_scale, kShift);
           l[x][j] *= corr[j];
 #pragma unroll
-          for (int c = 0; c < DC; ++c) cor[x][c][j] *= corr[j];
+          for (int c = 0; c < DC; ++c) {
+            cor[x][c][j] *= corr[j];
+            if (PAGED) psum[PAGED ? c : 0][x][j] *= corr[j];
+          }
         }
 #pragma unroll
         for (int c = 0; c < DC; ++c)
@@ -327,76 +463,94 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
       }
     }
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float mu = m[x][e & 1] == -INFINITY ? 0.f : m[x][e & 1];
-        sc[x][e] = ex2f(sc[x][e] - mu);
-        l[x][e & 1] += sc[x][e];
-      }
-
-    // ---- O^T += V^T P^T ----
-    uint32_t pb[NT][2];
-    if (!PAGED) {
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pb[x][h] = transpose8x8(PF16 ? pack_f16x2(sc[x][2 * h], sc[x][2 * h + 1])
-                                       : pack_bf16x2(sc[x][2 * h], sc[x][2 * h + 1]));
-    }
-#pragma unroll
-    for (int c = 0; c < DC; ++c) {
-      if (PAGED) {
-        float s[2], z[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          s[h] = __low2float(vsc[c][h]);
-          z[h] = fmaf(8.f, s[h], __high2float(vsc[c][h]));
+        for (int e = 0; e < 4; ++e) {
+          sc[kb][x][e] = ex2f(fmaf(sc[kb][x][e], score_scale, negm[x][e & 1]));
+          l[x][e & 1] += sc[kb][x][e];
         }
+
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      uint32_t pb[NT][2];
+      if (!PAGED) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
+          for (int h = 0; h < 2; ++h)
+            pb[x][h] = transpose8x8(PF16 ? pack_f16x2(sc[kb][x][2 * h], sc[kb][x][2 * h + 1])
+                                         : pack_bf16x2(sc[kb][x][2 * h], sc[kb][x][2 * h + 1]));
+      }
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        if (PAGED) {
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float e0 = sc[x][2 * h] * s[h], e1 = sc[x][2 * h + 1] * s[h];
-            float g0 = sc[x][2 * h] * z[h], g1 = sc[x][2 * h + 1] * z[h];
-            if (!full) {  // scales of slots that hold nothing may be NaN
-              if (sc[x][2 * h] == 0.f) e0 = g0 = 0.f;
-              if (sc[x][2 * h + 1] == 0.f) e1 = g1 = 0.f;
+            const float2 vsc =
+                __half22float2(*reinterpret_cast<const __half2*>(st + n * (4 * DC) + Ring::VS + ((kb * 16 + 8 * h) * DC + c) * 4));
+            const float f = vsc.x, z = fmaf(8.f, vsc.x, vsc.y);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              cor[x][c][0] = fmaf(sc[kb][x][2 * h], z, cor[x][c][0]);
+              cor[x][c][1] = fmaf(sc[kb][x][2 * h + 1], z, cor[x][c][1]);
+              pb[x][h] = transpose8x8(pack_bf16x2(sc[kb][x][2 * h] * f, sc[kb][x][2 * h + 1] * f));
             }
-            cor[x][c][0] += g0;
-            cor[x][c][1] += g1;
-            pb[x][h] = transpose8x8(pack_bf16x2(e0, e1));
           }
-        const uint32_t lo0 = __byte_perm(vq[c][0], vq[c][1], 0x5410), hi0 = __byte_perm(vq[c][0], vq[c][1], 0x7632);
-        const uint32_t lo1 = __byte_perm(vq[c][2], vq[c][3], 0x5410), hi1 = __byte_perm(vq[c][2], vq[c][3], 0x7632);
+          const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w0 = j < 2 ? lo0 : hi0, w1 = j < 2 ? lo1 : hi1;
-          const int q = (2 * j) & 3;
-          const uint32_t a[4] = {code_pair_centred(w0, q), code_pair_centred(w0, q + 1), code_pair_centred(w1, q),
-                                 code_pair_centred(w1, q + 1)};
+          for (int x = 0; x < NT; ++x) mma16816<false>(psum[PAGED ? c : 0][x], ones, pb[x][0], pb[x][1]);
+          uint32_t vq[4];
 #pragma unroll
-          for (int x = 0; x < NT; ++x) mma16816<false>(o[c][j][x], a, pb[x][0], pb[x][1]);
-        }
-      } else {
-        const uint32_t* e0 = reinterpret_cast<const uint32_t*>(&vd[c][0]);
-        const uint32_t* e1 = reinterpret_cast<const uint32_t*>(&vd[c][1]);
-        const uint32_t* e2 = reinterpret_cast<const uint32_t*>(&vd[c][2]);
-        const uint32_t* e3 = reinterpret_cast<const uint32_t*>(&vd[c][3]);
+          for (int e = 0; e < 4; ++e)
+            vq[e] = *reinterpret_cast<const uint32_t*>(st + voff[c] + (kb * 16 + (e & 1) * 8 + (e >> 1) * 4) * Ring::ROW);
+          const uint32_t lo0 = __byte_perm(vq[0], vq[1], 0x5410), hi0 = __byte_perm(vq[0], vq[1], 0x7632);
+          const uint32_t lo1 = __byte_perm(vq[2], vq[3], 0x5410), hi1 = __byte_perm(vq[2], vq[3], 0x7632);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t a[4] = {__byte_perm(e0[j], e1[j], 0x5410), __byte_perm(e0[j], e1[j], 0x7632),
-                                 __byte_perm(e2[j], e3[j], 0x5410), __byte_perm(e2[j], e3[j], 0x7632)};
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w0 = j < 2 ? lo0 : hi0, w1 = j < 2 ? lo1 : hi1;
+            const int q = (2 * j) & 3;  // codes 2j and 2j + 1 at bits 4q, 4q + 4 of both halves
+            const uint32_t a[4] = {code_pair(w0, w0 >> 8, q), code_pair(w0, w0 >> 8, q + 1), code_pair(w1, w1 >> 8, q),
+                                   code_pair(w1, w1 >> 8, q + 1)};
 #pragma unroll
-          for (int x = 0; x < NT; ++x) mma16816<PF16>(o[c][j][x], a, pb[x][0], pb[x][1]);
+            for (int x = 0; x < NT; ++x) mma16816<false>(o[c][j][x], a, pb[x][0], pb[x][1]);
+          }
+        } else {
+          uint32_t e0[4], e1[4], e2[4], e3[4];
+          auto row = [&](int r, uint32_t (&w)[4]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(st + Ring::V + (kb * 16 + r) * Ring::ROW + (((c * 8 + n) ^ (r & 7)) * 16));
+            w[0] = x.x;
+            w[1] = x.y;
+            w[2] = x.z;
+            w[3] = x.w;
+          };
+          row(2 * t, e0);
+          row(2 * t + 1, e1);
+          row(2 * t + 8, e2);
+          row(2 * t + 9, e3);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a[4] = {__byte_perm(e0[j], e1[j], 0x5410), __byte_perm(e0[j], e1[j], 0x7632),
+                                   __byte_perm(e2[j], e3[j], 0x5410), __byte_perm(e2[j], e3[j], 0x7632)};
+#pragma unroll
+            for (int x = 0; x < NT; ++x) mma16816<PF16>(o[c][j][x], a, pb[x][0], pb[x][1]);
+          }
         }
       }
     }
-    load_v(i + kSplitWarps, page_next);
-    page = page_next;
-    page_next = page_of(i + 2 * kSplitWarps);
+    __syncwarp();
+    int next = stage + Ring::STAGES - 1;  // the stage that the step before this one emptied
+    if (next >= Ring::STAGES) next -= Ring::STAGES;
+    load(i + (Ring::STAGES - 1) * kSplitWarps, row_next, next);
+    if (++stage == Ring::STAGES) stage = 0;
+    if (PAGED) {
+      missing_steps = (missing_steps | (uint32_t)(row_next == kNoRow) << (Ring::STAGES - 1)) >> 1;
+      row_next = cache_row(i + Ring::STAGES * kSplitWarps);
+    }
   }
+  cp_async_wait<0>();
 
   // ---- join the lanes (sums), then the warps ----
 #pragma unroll
@@ -410,7 +564,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
 #pragma unroll
           for (int c = 0; c < DC; ++c) cor[x][c][j] += __shfl_xor_sync(0xffffffffu, cor[x][c][j], d);
       }
-      if (n == 0) sml[warp][8 * x + 2 * t + j] = make_float2(m[x][j], l[x][j]);
+      if (PAGED)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) cor[x][c][j] = fmaf(-8.f, psum[PAGED ? c : 0][x][j], cor[x][c][j]);
+      if (n == 0) sml[warp][8 * x + 2 * t + j] = make_float2(m[x][j] * score_scale, PAGED ? l[x][j] / kPow64 : l[x][j]);
     }
   __syncthreads();
   float f[NT][2];
@@ -421,42 +578,60 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Attn
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, sml[w][8 * x + 2 * t + j].x);
-      f[x][j] = m[x][j] == -INFINITY ? 0.f : ex2f(m[x][j] - top);
+      f[x][j] = m[x][j] == -INFINITY ? 0.f : ex2f(m[x][j] * score_scale - top);
     }
-  for (int w = 0; w < kSplitWarps; ++w) {
-    if (warp == w) {
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float* dst = &so[8 * x + 2 * t + (e & 1)][64 * c + 8 * n + 2 * j + (e >> 1)];
-              const float v = (o[c][j][x][e] + (PAGED ? cor[x][c][e & 1] : 0.f)) * f[x][e & 1];
-              *dst = w ? *dst + v : v;
-            }
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < nr * DP; i += kSplitWarps * 32) {
-    const int r = i / DP, d = i % DP;
-    if (d >= p.D) continue;
-    float top = -INFINITY;
+  if (threadIdx.x < nr) {  // maximum and sum of the CTA's share, or 1 / sum
+    const int r = threadIdx.x;
+    float top = -INFINITY, ls = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, sml[w][r].x);
-    float ls = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w)
       if (sml[w][r].x != -INFINITY) ls = fmaf(sml[w][r].y, ex2f(sml[w][r].x - top), ls);
+    if (gridDim.x > 1) p.part_ml[out_row + r] = make_float2(top, ls);
+    sinv[r] = ls > 0.f ? 1.f / ls : 0.f;
+  }
+  __syncwarp();
+  float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int c = 0; c < DC; ++c)
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v[8];  // channels 64 c + 8 n ..
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = o[c][j][x][2 * e + r];  // codes at bits 4..7 (rows n + 8) count 16 times
+            if (PAGED) y = fmaf(y, e ? kPow69 / 16.f : kPow69, cor[x][c][r] / kPow64);
+            v[2 * j + e] = y * f[x][r];
+          }
+        float4* dst = reinterpret_cast<float4*>(mine + (8 * x + 2 * t + r) * (DP + 4) + 64 * c + 8 * n);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nr * (DP / 4); i += kSplitWarps * 32) {
+    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(split_smem + w * Ring::BYTES) + r * (DP + 4) + d);
+      x[0] += y.x;
+      x[1] += y.y;
+      x[2] += y.z;
+      x[3] += y.w;
+    }
+    if (d >= p.D) continue;  // D is a multiple of 8
     if (gridDim.x > 1) {
-      p.part_o[(out_row + r) * p.D + d] = so[r][d];
-      if (d == 0) p.part_ml[out_row + r] = make_float2(top, ls);
+      *reinterpret_cast<float4*>(p.part_o + (out_row + r) * p.D + d) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
       const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
-      static_cast<T*>(p.o)[b * p.os[0] + h * p.os[1] + qi * p.os[2] + d * p.os[3]] =
-          from_f32<T>(ls > 0.f ? so[r][d] / ls : 0.f);
+      T* dst = static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + qi * p.os[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[(d + j) * p.os[3]] = from_f32<T>(x[j] * sinv[r]);
     }
   }
 }
@@ -476,6 +651,32 @@ int split_count(int64_t bk, int64_t rows, int64_t keys) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 512));
 }
 
+template <bool F16, bool PAGED, int DC, int NT, int KB>
+static int split_launch_kernel(AttnParams& p, dim3 grid, cudaStream_t st) {
+  constexpr int smem = kSplitWarps * SplitRing<PAGED, DC, KB>::BYTES;
+  auto kern = attn_split_kernel<F16, PAGED, DC, NT, KB>;
+  static int resident[64] = {};  // CTAs an SM holds
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& res = resident[dev & 63];
+  if (!res) {
+    int n = 0;
+    int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                        "attention split smem attribute");
+    if (!rc)
+      rc = cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kSplitWarps * 32, smem),
+                      "attention split occupancy");
+    if (rc) return rc;
+    res = std::max(n, 1);
+  }
+  // chunks for three waves over the codes (arithmetic counts, the waves even out) and one and a half over 16-bit
+  // rows, where a chunk's start costs more: 24 sequences of 4096..16384 codes take 111, 83, 83, 79, 80 us with 2, 3,
+  // 8, 12, 16 CTAs an SM (4 resident), 8 sequences of 4096 16-bit keys 33, 32, 35, 37 with 2, 3, 4, 8 (2 resident)
+  p.target = num_sms() * (PAGED ? 3 * res : (3 * res + 1) / 2);
+  kern<<<grid, kSplitWarps * 32, smem, st>>>(p);
+  return check_launch("attention_split");
+}
+
 template <bool F16, bool PAGED, int DC>
 static int split_launch_dc(AttnParams& p, cudaStream_t st) {
   const int tr = split_tile_rows(p.rows);
@@ -483,10 +684,15 @@ static int split_launch_dc(AttnParams& p, cudaStream_t st) {
   if ((int64_t)p.B * p.Hkv > 65535 || tiles > 65535)
     return fail(MT_ERR_UNSUPPORTED, "window_attention: batch * key heads or rows past the grid");
   dim3 grid((unsigned)p.splits, (unsigned)(p.B * p.Hkv), (unsigned)tiles);
-  p.target = 8 * num_sms();
-  if (tr == 8) attn_split_kernel<F16, PAGED, DC, 1><<<grid, kSplitWarps * 32, 0, st>>>(p);
-  else attn_split_kernel<F16, PAGED, DC, 2><<<grid, kSplitWarps * 32, 0, st>>>(p);
-  return check_launch("attention_split");
+  // two blocks a step where pages allow it and the scales fit one instruction: control and votes are shared
+  // (cache4_batch of the benchmark, pages of 64)
+  constexpr int KB2 = PAGED && DC <= 2 ? 2 : 1;
+  if (KB2 == 2 && p.page_shift >= 5) {
+    return tr == 8 ? split_launch_kernel<F16, PAGED, DC, 1, KB2>(p, grid, st)
+                   : split_launch_kernel<F16, PAGED, DC, 2, KB2>(p, grid, st);
+  }
+  return tr == 8 ? split_launch_kernel<F16, PAGED, DC, 1, 1>(p, grid, st)
+                 : split_launch_kernel<F16, PAGED, DC, 2, 1>(p, grid, st);
 }
 
 template <bool F16, bool PAGED>
@@ -500,6 +706,8 @@ static int split_launch(AttnParams& p, cudaStream_t st) {
 }
 
 int run_split_attention(AttnParams& p, int dtype, bool paged, cudaStream_t st) {
+  if (paged && ((int64_t)p.num_pages * p.Hkv << (p.page_shift - 4)) >= 0xffffffffLL)
+    return fail(MT_ERR_UNSUPPORTED, "kv_cache4_attention: more than 2^36 tokens and heads in the cache");
   if (dtype == MT_F16) return paged ? split_launch<true, true>(p, st) : split_launch<true, false>(p, st);
   return paged ? split_launch<false, true>(p, st) : split_launch<false, false>(p, st);
 }
