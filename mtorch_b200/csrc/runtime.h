@@ -129,6 +129,7 @@ int read_status_gemm(int clear);
 int run_wait_timeout_selftest(long long budget_cycles, cudaStream_t st);
 int read_status_attention(int clear);
 int read_status_norm(int clear);
+int read_status_window_attention(int clear);
 #define MT_STATUS_READER(name)                                                   \
   int name(int clear) {                                                          \
     int v = 0;                                                                   \

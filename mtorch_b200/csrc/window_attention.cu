@@ -274,11 +274,16 @@ static bool aligned16(const void* base, const int64_t* s, int64_t D) {
   return s[3] == 1 && D % 8 == 0 && (uintptr_t)base % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
 }
 
+// The tensor-core kernel computes tiles of 128 queries of a head whatever their number; the split kernel reads the
+// keys anew for each 16 rows of a key head.
+static bool takes_sm100(const mt_window_attention_desc& d) { return d.Sq > 32 && window_sm100_takes(d); }
+
 static bool takes_split(const mt_window_attention_desc& d) {
   return d.dtype != MT_F32 && aligned16(d.k, d.k_strides, d.D) && aligned16(d.v, d.v_strides, d.D);
 }
 
 static int window_splits(const mt_window_attention_desc& d) {
+  if (takes_sm100(d)) return 1;
   if (takes_split(d))
     return split_count(d.B * d.Hkv, d.Sq * (d.H / d.Hkv), span_keys(d.Sk, d.Sq, d.causal, d.window, d.sinks));
   return rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks);
@@ -394,6 +399,7 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
   if (ws_bytes < window_attention_workspace(d) || (p.splits > 1 && !ws))
     return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
   bind_workspace(p, ws);
+  if (takes_sm100(d)) return run_window_sm100(d, p, st);
   if (takes_split(d)) {
     p.q_vec = aligned16(d.q, d.q_strides, d.D);
     rc = run_split_attention(p, d.dtype, false, st);

@@ -82,4 +82,8 @@ __device__ __forceinline__ BlockList block_list(const AttnParams& p, const SeqPo
 int split_count(int64_t bk, int64_t rows, int64_t keys);
 int run_split_attention(AttnParams& p, int dtype, bool paged, cudaStream_t st);
 
+// window_attention_sm100.cu: many queries over 16-bit keys, head dims up to 128
+bool window_sm100_takes(const mt_window_attention_desc& d);
+int run_window_sm100(const mt_window_attention_desc& d, const AttnParams& a, cudaStream_t st);
+
 }  // namespace mt
