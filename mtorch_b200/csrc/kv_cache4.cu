@@ -13,7 +13,7 @@ struct Cache4Params {
   int64_t table_stride;
   int max_pages, page_shift, num_pages;
   int Hkv, D, T;
-  int64_t items;  // B * T * Hkv * D / 8
+  int items;  // T * Hkv * D / 8: words of one sequence
   const int32_t* starts;
   int32_t* words[2];
   __half2* scales[2];  // (scale, zero)
@@ -51,17 +51,14 @@ __device__ __forceinline__ void load8(const T* src, int64_t st, bool vec, float 
 
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int kv = blockIdx.y;
-  const int W = p.D / 8;
-  const bool live = idx < p.items;  // whole groups of 8 threads are live or not
-  const int64_t i = live ? idx : 0;
-  const int w = (int)(i % W);
-  int64_t r = i / W;
-  const int h = (int)(r % p.Hkv);
-  r /= p.Hkv;
-  const int t = (int)(r % p.T);
-  const int64_t b = r / p.T;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const int kv = blockIdx.y & 1;
+  const int64_t b = blockIdx.y >> 1;
+  const uint32_t W = p.D / 8;
+  const bool live = idx < (uint32_t)p.items;  // whole groups of 8 threads are live or not
+  const uint32_t i = live ? idx : 0;
+  const uint32_t r = i / W, w = i - r * W;
+  const int t = r / (uint32_t)p.Hkv, h = r - (uint32_t)t * p.Hkv;
   const int64_t row = live ? cache4_row(p, b, h, t) : -1;
   const T* src = static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
                  (int64_t)w * 8 * p.st[kv][3];
@@ -95,16 +92,13 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p
 
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int kv = blockIdx.y;
-  if (idx >= p.items) return;
-  const int W = p.D / 8;
-  const int w = (int)(idx % W);
-  int64_t r = idx / W;
-  const int t = (int)(r % p.T);
-  r /= p.T;
-  const int h = (int)(r % p.Hkv);
-  const int64_t b = r / p.Hkv;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const int kv = blockIdx.y & 1;
+  const int64_t b = blockIdx.y >> 1;
+  if (idx >= (uint32_t)p.items) return;
+  const uint32_t W = p.D / 8;
+  const uint32_t r = idx / W, w = idx - r * W;
+  const int h = r / (uint32_t)p.T, t = r - (uint32_t)h * p.T;
   const int64_t row = cache4_row(p, b, h, t);
   uint32_t word = 0;
   float s = 0.f, z = 0.f;
@@ -158,7 +152,8 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   p.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
   p.num_pages = (int)c.num_pages;
   p.Hkv = (int)c.Hkv; p.D = (int)c.D; p.T = (int)T;
-  p.items = B * T * c.Hkv * (c.D / 8);
+  if (B > 32767 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
+  p.items = (int)(T * c.Hkv * (c.D / 8));
   p.starts = starts;
   p.words[0] = c.k_words; p.words[1] = c.v_words;
   p.scales[0] = static_cast<__half2*>(c.k_scales); p.scales[1] = static_cast<__half2*>(c.v_scales);
@@ -170,7 +165,6 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
     p.vec = p.vec && s[3] == 1 && (uintptr_t)(i ? v : k) % 16 == 0;
     for (int j = 0; j < 3; ++j) p.vec = p.vec && (s[j] * es) % 16 == 0;
   }
-  if ((p.items + 255) / 256 > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "%s: too many elements", what);
   return MT_OK;
 }
 
@@ -179,9 +173,9 @@ int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks
                          int64_t max_pages, const int32_t* starts, cudaStream_t st) {
   Cache4Params p{};
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_append");
-  if (rc || p.items == 0) return rc;
+  if (rc || B == 0 || p.items == 0) return rc;
   p.in[0] = k; p.in[1] = v;
-  dim3 grid((unsigned)((p.items + 255) / 256), 2);
+  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
   switch (dtype) {
     case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
     case MT_BF16: cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
@@ -195,9 +189,9 @@ int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* 
                        const int32_t* starts, cudaStream_t st) {
   Cache4Params p{};
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_read");
-  if (rc || p.items == 0) return rc;
+  if (rc || B == 0 || p.items == 0) return rc;
   p.out[0] = k; p.out[1] = v;
-  dim3 grid((unsigned)((p.items + 255) / 256), 2);
+  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
   switch (dtype) {
     case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;
     case MT_BF16: cache4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;

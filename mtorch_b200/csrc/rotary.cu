@@ -70,16 +70,118 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryParams p, c
   }
 }
 
+template <int BYTES> struct RotaryVec;
+template <> struct RotaryVec<16> { using type = uint4; };
+template <> struct RotaryVec<8> { using type = uint2; };
+template <> struct RotaryVec<4> { using type = uint32_t; };
+
+// VEC elements (up to 16 bytes) at a time.  Split pairs: a thread holds channels c .. c + VEC - 1 and their partners
+// `pairs` further on (pairs is a multiple of VEC), or VEC copied channels.  Interleaved pairs: a thread holds VEC
+// channels, VEC / 2 pairs, those at and past `pairs` copied.  The angles of a (token, channel) are computed once
+// for all the heads the thread walks through, four heads' loads ahead of their use.
+template <typename T, int VEC, bool INTER>
+__global__ void __launch_bounds__(256) rotary_vec_kernel(const RotaryParams p) {
+  using V = typename RotaryVec<VEC * sizeof(T)>::type;
+  constexpr int NP = INTER ? VEC / 2 : VEC;  // pairs of a thread
+  constexpr int NV = INTER ? 1 : 2;          // vectors of a thread
+  const int items = INTER ? p.D / VEC : (p.D - p.pairs) / VEC;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t tok = idx / items;
+  if (tok >= p.tokens) return;
+  const int c = (idx - tok * items) * VEC;
+  const int64_t b = tok / (uint32_t)p.S;
+  const int s = tok - (uint32_t)b * p.S;
+  // first channel of each vector; copied channels of split pairs follow the second halves
+  const bool turns = INTER ? c / 2 < p.pairs : c < p.pairs;
+  const int d0 = INTER || turns ? c : c + p.pairs, d1 = c + p.pairs;
+  float sn[NP], cs[NP];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int pair = INTER ? c / 2 + j : c + j;
+    sn[j] = 0.f;
+    cs[j] = 1.f;
+    if (pair < p.pairs) rotary_sincos(p, b, s, pair, sn[j], cs[j]);
+  }
+  const int h0 = blockIdx.y * p.heads_per_block, h1 = min(p.Hq + p.Hk, h0 + p.heads_per_block);
+  constexpr int U = 4;  // heads in flight
+  for (int h = h0; h < h1; h += U) {
+    V in[U][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int hh = min(h + u, h1 - 1), w = hh < p.Hq ? 0 : 1;
+      const T* src = static_cast<const T*>(p.in[w]) + b * p.is[w][0] + (w ? hh - p.Hq : hh) * p.is[w][1] + s * p.is[w][2];
+      in[u][0] = *reinterpret_cast<const V*>(src + d0);
+      if (!INTER && turns) in[u][NV - 1] = *reinterpret_cast<const V*>(src + d1);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;
+      const int hh = h + u, w = hh < p.Hq ? 0 : 1;
+      T* dst = static_cast<T*>(p.out[w]) + b * p.os[w][0] + (w ? hh - p.Hq : hh) * p.os[w][1] + s * p.os[w][2];
+      if (turns) {
+        T* e = reinterpret_cast<T*>(&in[u][0]);
+        T* f = reinterpret_cast<T*>(&in[u][NV - 1]);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          T& xr = INTER ? e[2 * j] : e[j];
+          T& yr = INTER ? e[2 * j + 1] : f[j];
+          float x = to_f32<T>(xr), y = to_f32<T>(yr);
+          rotary_turn(x, y, sn[j], cs[j]);
+          if (!INTER || c / 2 + j < p.pairs) {
+            xr = from_f32<T>(x);
+            yr = from_f32<T>(y);
+          }
+        }
+        if (!INTER) *reinterpret_cast<V*>(dst + d1) = in[u][NV - 1];
+      }
+      *reinterpret_cast<V*>(dst + d0) = in[u][0];
+    }
+  }
+}
+
+// Largest vector (elements) that every row of the tensors allows; 1: none.
+static int rotary_vec(const mt_rotary_desc& d) {
+  const int es = dtype_size(d.dtype);
+  for (int vec = 16 / es; vec > 1; vec /= 2) {
+    bool ok = d.D % vec == 0 && (d.interleaved || d.pairs % vec == 0);
+    for (int i = 0; i < 4; ++i) {
+      const bool second = i & 1;
+      if (second && !d.Hk) continue;
+      if (!second && !d.Hq) continue;
+      const void* base = i < 2 ? (second ? d.k : d.q) : (second ? d.k_out : d.q_out);
+      const int64_t* st = i < 2 ? (second ? d.k_strides : d.q_strides) : (second ? d.k_out_strides : d.q_out_strides);
+      ok = ok && st[3] == 1 && (uintptr_t)base % (vec * es) == 0 && st[0] % vec == 0 && st[1] % vec == 0 && st[2] % vec == 0;
+    }
+    if (ok) return vec;
+  }
+  return 1;
+}
+
+template <typename T, int VEC>
+static void rotary_vec_launch(bool inter, dim3 grid, const RotaryParams& p, cudaStream_t st) {
+  if (inter) rotary_vec_kernel<T, VEC, true><<<grid, 256, 0, st>>>(p);
+  else rotary_vec_kernel<T, VEC, false><<<grid, 256, 0, st>>>(p);
+}
+
 template <typename T>
 static int rotary_launch(const mt_rotary_desc& d, RotaryParams& p, cudaStream_t st) {
   const int heads = p.Hq + p.Hk;
-  const int64_t items = p.tokens * (p.D - p.pairs);
+  const int vec = p.tokens * p.D < UINT32_MAX - 256 ? rotary_vec(d) : 1;  // (the vector kernel counts in 32 bits)
+  const int64_t items = p.tokens * (vec > 1 ? (d.interleaved ? p.D / vec : (p.D - p.pairs) / vec) : p.D - p.pairs);
   const int64_t blocks = (items + 255) / 256;
   if (blocks > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "rotary: too many elements");
-  int64_t parts = std::min<int64_t>(heads, std::max<int64_t>(1, (4LL * num_sms() + blocks - 1) / blocks));
+  // heads are shared out over CTAs until the GPU is full: few tokens leave nothing else to share
+  int64_t parts = std::min<int64_t>(heads, std::max<int64_t>(1, (8LL * num_sms() + blocks - 1) / blocks));
   p.heads_per_block = (int)((heads + parts - 1) / parts);
   dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block));
-  rotary_any_kernel<T><<<grid, 256, 0, st>>>(p, d.interleaved != 0);
+  const bool inter = d.interleaved != 0;
+  if (vec > 1) {
+    if (vec * (int)sizeof(T) == 16) rotary_vec_launch<T, 16 / sizeof(T)>(inter, grid, p, st);
+    else if (vec * (int)sizeof(T) == 8) rotary_vec_launch<T, 8 / sizeof(T)>(inter, grid, p, st);
+    else if constexpr (sizeof(T) == 2) rotary_vec_launch<T, 2>(inter, grid, p, st);
+  } else {
+    rotary_any_kernel<T><<<grid, 256, 0, st>>>(p, inter);
+  }
   return check_launch("rotary");
 }
 
