@@ -26,6 +26,7 @@ constexpr int kWaThreads = 384;  // producer, MMA issuer, two idle warps; two so
 // registers: 384 threads start with 168 each; 128 * 72 + 256 * 216 = 384 * 168
 constexpr int kWaRegsIssue = 72, kWaRegsSoftmax = 216;
 constexpr float kWaLazy = 8.0f;
+constexpr int kWaPoly = 2;  // of 8 pairs of exponentials, those on the FMA pipe
 
 struct WaParams {
   AttnParams a;
@@ -61,18 +62,56 @@ __device__ __forceinline__ uint64_t wa_add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// maximum of 128 values, four independent chains
+// maximum of 128 values, eight independent chains
 __device__ __forceinline__ float wa_max128(const uint32_t (&r)[128]) {
-  float m[4];
+  float m[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(r[i]);
 #pragma unroll
-  for (int k = 4; k + 8 <= 128; k += 8)
+  for (int k = 8; k + 16 <= 128; k += 16)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = wa_max3(m[i], __uint_as_float(r[k + i]), __uint_as_float(r[k + 4 + i]));
+    for (int i = 0; i < 8; ++i) m[i] = wa_max3(m[i], __uint_as_float(r[k + i]), __uint_as_float(r[k + 8 + i]));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], __uint_as_float(r[124 + i]));
-  return fmaxf(wa_max3(m[0], m[1], m[2]), m[3]);
+  for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], __uint_as_float(r[120 + i]));
+  return wa_max3(wa_max3(m[0], m[1], m[2]), wa_max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+
+// 2^x of two values on the FMA pipe: x = i + f with |f| <= 1/2, a polynomial for 2^f (minimax in relative error by the
+// Remez exchange: 7.5e-5 for degree 3, 2.6e-6 for degree 4, a fraction of P's rounding to bf16 / f16), i added to
+// the exponent.  Below 2^-126 it stays there.
+template <bool F16>
+__device__ __forceinline__ void wa_exp2_poly(float& a0, float& a1) {
+  a0 = fmaxf(a0, -126.f);
+  a1 = fmaxf(a1, -126.f);
+  const uint64_t x = wa_pack2(a0, a1);
+  const uint64_t t = wa_add2(x, wa_pack2(12582912.f, 12582912.f));  // 1.5 * 2^23: rounds to a whole number
+  const uint64_t i = wa_add2(t, wa_pack2(-12582912.f, -12582912.f));
+  const uint64_t f = wa_fma2(i, wa_pack2(-1.f, -1.f), x);
+  uint64_t y;
+  if (F16) {
+    y = wa_fma2(wa_pack2(0.009570102f, 0.009570102f), f, wa_pack2(0.05591786f, 0.05591786f));
+    y = wa_fma2(y, f, wa_pack2(0.24024745f, 0.24024745f));
+    y = wa_fma2(y, f, wa_pack2(0.69312181f, 0.69312181f));
+    y = wa_fma2(y, f, wa_pack2(0.99999926f, 0.99999926f));
+  } else {
+    y = wa_fma2(wa_pack2(0.05517167f, 0.05517167f), f, wa_pack2(0.24261112f, 0.24261112f));
+    y = wa_fma2(y, f, wa_pack2(0.69326099f, 0.69326099f));
+    y = wa_fma2(y, f, wa_pack2(0.99992807f, 0.99992807f));
+  }
+  float t0, t1;
+  wa_unpack2(t, t0, t1);
+  wa_unpack2(y, a0, a1);
+  a0 = __uint_as_float(__float_as_uint(a0) + (__float_as_uint(t0) << 23));
+  a1 = __uint_as_float(__float_as_uint(a1) + (__float_as_uint(t1) << 23));
+}
+
+// bits c of the 32 columns from `base` on that a row sees
+__device__ __forceinline__ uint32_t wa_row_bits(const RowKeys& rk, int base) {
+  const int lo = rk.lo - base, hi = rk.hi - base, sk = rk.sk - base;
+  const uint32_t ge = lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo;
+  const uint32_t le = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
+  const uint32_t first = sk <= 0 ? 0u : sk >= 32 ? ~0u : (1u << sk) - 1u;
+  return (ge & le) | first;
 }
 
 __device__ __forceinline__ void wa_tmem_st32(uint32_t taddr, const uint32_t* r) {
@@ -86,26 +125,45 @@ __device__ __forceinline__ void wa_tmem_st32(uint32_t taddr, const uint32_t* r) 
       : "memory");
 }
 
-// D (+)= A (TMEM, 16-bit, two K elements a column) * B (shared memory descriptor)
-__device__ __forceinline__ void wa_umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// Products issued by the elected lane of a warp that runs as one: addresses, loop counters and descriptors then stay
+// in uniform registers, which the instruction takes its operands from.  A descriptor is passed as its low word; the
+// high word is the same for all operands here (8 rows of 128 bytes = 1024, version, 128-byte swizzle).
+constexpr uint32_t kWaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// low words: rows along K (Q, K: the next 64 channels are another tile); rows along N (V: 64 channels of one key are
+// 128 bytes, the next 64 channels lie `chunk` bytes on)
+__device__ __forceinline__ uint32_t wa_desc_k(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t wa_desc_n(uint32_t addr, uint32_t chunk) {
+  return ((addr & 0x3FFFF) >> 4) | ((chunk >> 4) << 16);
+}
+// D (+)= A B^T, both in shared memory
+__device__ __forceinline__ void wa_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                          uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, q;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n mov.b64 da, {%1, %6};\n"
+      " mov.b64 db, {%2, %6};\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(leader), "n"(kWaDescHi)
       : "memory");
 }
-
-// Operand whose rows along N are contiguous (V: 64 channels of one key = 128 bytes, swizzled; 8 keys = 1024 bytes):
-// the next 64 channels lie `chunk` bytes on, the next 8 keys 1024.
-__device__ __forceinline__ uint64_t wa_desc_mn(uint32_t addr, uint32_t chunk) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(chunk >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;  // SWIZZLE_128B
-  return d;
+// D (+)= A B with A in TMEM (16-bit, two K elements a column)
+__device__ __forceinline__ void wa_mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                          uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n mov.b64 db, {%2, %6};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(leader), "n"(kWaDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void wa_commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t wa_elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(r));
+  return r;
 }
 
 template <int DP>
@@ -141,8 +199,8 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   uint64_t* v_full = k_empty + Cfg::STAGES_K;
   uint64_t* v_empty = v_full + Cfg::STAGES_V;
   uint64_t* s_full = v_empty + Cfg::STAGES_V;     // [2]
-  uint64_t* p_full = s_full + 2;                  // [2]
-  uint64_t* o_done = p_full + 2;                  // [2]
+  uint64_t* p_full = s_full + 2;                  // [2][2]: the first and the second 64 keys of P_x
+  uint64_t* o_done = p_full + 4;                  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -177,7 +235,8 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], kWaTile);
+      mbar_init(&p_full[2 * x], kWaTile);
+      mbar_init(&p_full[2 * x + 1], kWaTile);
       mbar_init(&o_done[x], 1);
     }
     *abort_flag = 0;
@@ -254,70 +313,80 @@ __global__ void __launch_bounds__(kWaThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0 && bl.count > 0) {
-      const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-      bool ok = mbar_wait(q_full, 0, 74, abort_flag);
+    // ---------------- MMA issuer (the whole warp runs it, one lane issues) ----------------
+    if (bl.count > 0) {
+      const uint32_t leader = wa_elect();
+      const uint32_t q_lo = wa_desc_k(smem_u32(sQ)), k_lo = wa_desc_k(smem_u32(sK)), v_lo = wa_desc_n(smem_u32(sV), Cfg::CHUNK);
+      const BlockList t0 = tiles_of(0), t1 = tiles_of(1);
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, site, abort_flag));
+      };
       int ks = 0, vs = 0;
       uint32_t kph = 0, vph = 0;
-      const BlockList tx[2] = {tiles_of(0), tiles_of(1)};
-      int done[2] = {0, 0};
+      int done0 = 0, done1 = 0;
       auto issue_s = [&](int x) {
+        const uint32_t qa = q_lo + x * (Cfg::TILE >> 4), ka = k_lo + ks * (Cfg::TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          umma_f16(tmem + x * 128, sdesc_sw128(q_addr + x * Cfg::TILE + (kk / 4) * Cfg::CHUNK + (kk % 4) * 32),
-                   sdesc_sw128(k_addr + ks * Cfg::TILE + (kk / 4) * Cfg::CHUNK + (kk % 4) * 32), idesc_s, kk > 0);
-        umma_commit(&s_full[x]);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const int off = ((kk / 4) * Cfg::CHUNK + (kk % 4) * 32) >> 4;
+          wa_mma_ss(tmem + x * 128, qa + off, ka + off, idesc_s, kk > 0, leader);
+        }
+        wa_commit(&s_full[x], leader);
       };
-      ok = ok && mbar_wait(&k_full[0], 0, 75, abort_flag);
+      // O_x += P_x V: the first half's products run under the second half's exponentials
+      auto issue_pv = [&](int x, int done) -> bool {
+        const uint32_t va = v_lo + vs * (Cfg::TILE >> 4);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(&p_full[2 * x + half], done & 1, 77)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+            wa_mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o, done > 0 || kk > 0, leader);
+        }
+        return true;
+      };
+      bool ok = wait(q_full, 0, 74) && wait(&k_full[0], 0, 75);
+      bool a0 = active(t0, 0), a1 = active(t1, 0);
       if (ok) {
         tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (active(tx[x], 0)) issue_s(x);
-        umma_commit(&k_empty[0]);
-        ks = 1 % Cfg::STAGES_K;
+        if (a0) issue_s(0);
+        if (a1) issue_s(1);
+        wa_commit(&k_empty[0], leader);
+        ks = 1;
       }
       for (int i = 0; ok && i < bl.count; ++i) {
-        bool have_k = false, have_v = false;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (ok && active(tx[x], i)) {
-            if (!have_v) ok = mbar_wait(&v_full[vs], vph, 76, abort_flag);
-            have_v = true;
-            ok = ok && mbar_wait(&p_full[x], done[x] & 1, 77, abort_flag);
-            if (!ok) continue;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < kWaTile / 16; ++kk)
-              wa_umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
-                         wa_desc_mn(v_addr + vs * Cfg::TILE + kk * 2048, Cfg::CHUNK), idesc_o, done[x] > 0 || kk > 0);
-            if (++done[x] == tx[x].count) umma_commit(&o_done[x]);
-          }
-          if (ok && active(tx[x], i + 1)) {
-            if (!have_k) ok = mbar_wait(&k_full[ks], kph, 78, abort_flag);
-            have_k = true;
-            if (!ok) continue;
-            tc_fence_after();
-            issue_s(x);
-          }
+        const bool more = i + 1 < bl.count;
+        const bool n0 = active(t0, i + 1), n1 = active(t1, i + 1);
+        // every tile has to arrive before its stage is handed back, also one that no row needs
+        ok = wait(&v_full[vs], vph, 76);
+        if (ok && a0) {
+          ok = issue_pv(0, done0);
+          if (++done0 == t0.count) wa_commit(&o_done[0], leader);
         }
-        // a tile that no row needed still has to arrive before its stage is handed back
-        if (ok && !have_v) ok = mbar_wait(&v_full[vs], vph, 76, abort_flag);
-        if (ok && !have_k && i + 1 < bl.count) ok = mbar_wait(&k_full[ks], kph, 78, abort_flag);
+        ok = ok && (!more || wait(&k_full[ks], kph, 78));
+        tc_fence_after();
+        if (ok && n0) issue_s(0);
+        if (ok && a1) {
+          ok = issue_pv(1, done1);
+          if (++done1 == t1.count) wa_commit(&o_done[1], leader);
+        }
+        if (ok && n1) issue_s(1);
         if (!ok) break;
-        umma_commit(&v_empty[vs]);
+        wa_commit(&v_empty[vs], leader);
         if (++vs == Cfg::STAGES_V) {
           vs = 0;
           vph ^= 1;
         }
-        if (i + 1 < bl.count) {
-          umma_commit(&k_empty[ks]);
+        if (more) {
+          wa_commit(&k_empty[ks], leader);
           if (++ks == Cfg::STAGES_K) {
             ks = 0;
             kph ^= 1;
           }
         }
+        a0 = n0;
+        a1 = n1;
       }
     }
   } else if (warp >= 4) {
@@ -330,9 +399,9 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem + x * 128 + lane_off, t_o = tmem + 256 + x * 128 + lane_off;
     const int q0 = qbase + x * kWaTile, qi = q0 + row;
-    const RowKeys rk = row_keys(p, sp, sp.start + min(qi, p.Sq - 1));
-    // keys that all rows of the tile see
-    const RowKeys ra = row_keys(p, sp, sp.start + q0), rz = row_keys(p, sp, sp.start + min(q0 + kWaTile, p.Sq) - 1);
+    // keys that all rows of the tile see: up to all_hi, from all_lo on or below all_sk
+    const RowKeys ra = row_keys(p, sp, sp.start + q0);
+    const int all_hi = ra.hi, all_sk = ra.sk, all_lo = row_keys(p, sp, sp.start + min(q0 + kWaTile, p.Sq) - 1).lo;
     const float sl = p.scale_log2;
     const uint64_t sl2 = wa_pack2(sl, sl);
     float m = -INFINITY, thr = -INFINITY, l = 0.f;
@@ -350,11 +419,15 @@ __global__ void __launch_bounds__(kWaThreads, 1)
       for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
       tmem_ld_wait();
       const int k0 = bl.block(i) * kWaTile;
-      if (!(k0 + kWaTile - 1 <= ra.hi && (k0 >= rz.lo || k0 + kWaTile - 1 < ra.sk))) {
-        const int lo = rk.lo - k0, hi = rk.hi - k0, sk = rk.sk - k0;
+      if (!(k0 + kWaTile - 1 <= all_hi && (k0 >= all_lo || k0 + kWaTile - 1 < all_sk))) {
+        const RowKeys rk = row_keys(p, sp, sp.start + min(qi, p.Sq - 1));
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (!((c >= lo && c <= hi) || c < sk)) r[c] = 0xff800000u;
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t bits = wa_row_bits(rk, k0 + w * 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!(bits & (1u << c))) r[w * 32 + c] = 0xff800000u;
+        }
       }
       const float top = wa_max128(r);
       if (__any_sync(0xffffffffu, top > thr)) {
@@ -384,22 +457,24 @@ __global__ void __launch_bounds__(kWaThreads, 1)
       uint64_t sum[2] = {wa_pack2(0.f, 0.f), wa_pack2(0.f, 0.f)};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = half * 32; c < half * 32 + 32; ++c) {  // in place: word c of P from scores 2c, 2c + 1
           float a0, a1;
-          wa_unpack2(wa_fma2(wa_pack2(__uint_as_float(r[half * 64 + 2 * c]), __uint_as_float(r[half * 64 + 2 * c + 1])),
-                             sl2, negm2), a0, a1);
-          a0 = wa_ex2(a0);
-          a1 = wa_ex2(a1);
+          wa_unpack2(wa_fma2(wa_pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sl2, negm2), a0, a1);
+          if (c % 8 < kWaPoly) {
+            wa_exp2_poly<F16>(a0, a1);
+          } else {
+            a0 = wa_ex2(a0);
+            a1 = wa_ex2(a1);
+          }
           sum[c & 1] = wa_add2(sum[c & 1], wa_pack2(a0, a1));
-          pk[c] = F16 ? pack_f16x2(a0, a1) : pack_bf16x2(a0, a1);
+          r[c] = F16 ? pack_f16x2(a0, a1) : pack_bf16x2(a0, a1);
         }
-        wa_tmem_st32(t_s + half * 32, pk);
+        wa_tmem_st32(t_s + half * 32, &r[half * 32]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * x + half]);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&p_full[x]);
       float s0, s1;
       wa_unpack2(wa_add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
@@ -408,7 +483,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     if (ok && k > 0) ok = mbar_wait(&o_done[x], 0, 80, abort_flag);
     if (ok && q0 < p.Sq) {
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = m > -INFINITY && l > 0.f ? 1.f / l : 0.f;  // m: -inf where the row saw no key
       const int64_t off = b * p.os[0] + h * p.os[1] + (int64_t)qi * p.os[2];
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
