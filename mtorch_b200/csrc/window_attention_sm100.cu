@@ -3,7 +3,7 @@
 //
 // One CTA = two tiles of 128 query rows of one (batch entry, head); the tiles of 128 keys that any of the rows
 // sees (the sinks' tiles, then the window's) stream through TMA rings of K and V, 128-byte swizzled.
-//   warp 0      producer: Q once, then K(0), K(j + 1), V(j), ..
+//   warp 0      producer: Q once and K(0) (before the barriers' first use), then K(j + 1), V(j), ..
 //   warp 1      MMA issuer: S_x = Q_x K^T into TMEM (fp32), then O_x += P_x V with P_x as the TMEM operand: it
 //               overwrites the low half of S_x's columns, so the probabilities never touch shared memory.
 //   warps 4..11 one softmax warpgroup per query tile, one row per thread: the row's 128 scores are read once into
@@ -205,8 +205,9 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, hk = h / p.g;
-  const int qbase = blockIdx.x * (2 * kWaTile);
+  // the last queries first: with a causal mask they have the most key tiles, and the short CTAs fill the end
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, hk = h / p.g;
+  const int qbase = (gridDim.y - 1 - blockIdx.y) * (2 * kWaTile);
   const SeqPos sp = seq_pos(p, b, false);
 
   // key tiles: of both query tiles together, and of each
@@ -241,6 +242,15 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     }
     *abort_flag = 0;
     fence_barrier_init();
+    if (bl.count > 0) {  // Q and the first K tile come while the rest is set up
+      mbar_arrive_expect_tx(q_full, 2 * Cfg::TILE);
+      for (int x = 0; x < 2; ++x)
+        for (int c = 0; c < CHUNKS; ++c)
+          tma_load_4d(sQ + x * Cfg::TILE + c * Cfg::CHUNK, &tmQ, q_full, c * 64, qbase + x * kWaTile, h, b);
+      mbar_arrive_expect_tx(&k_full[0], Cfg::TILE);
+      for (int c = 0; c < CHUNKS; ++c)
+        tma_load_4d(sK + c * Cfg::CHUNK, &tmK, &k_full[0], c * 64, bl.block(0) * kWaTile, hk, b);
+    }
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -254,16 +264,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWaRegsIssue));
   if (warp == 0) {
     // ---------------- producer ----------------
-    if (lane == 0 && bl.count > 0) {
-      tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      mbar_arrive_expect_tx(q_full, 2 * Cfg::TILE);
-      for (int x = 0; x < 2; ++x)
-        for (int c = 0; c < CHUNKS; ++c)
-          tma_load_4d(sQ + x * Cfg::TILE + c * Cfg::CHUNK, &tmQ, q_full, c * 64, qbase + x * kWaTile, h, b);
-    }
-    int ks = 0, vs = 0;
+    int ks = 1, vs = 0;
     uint32_t kph = 0, vph = 0;
     bool ok = true;
     auto load_k = [&](int i) {
@@ -280,7 +281,6 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         kph ^= 1;
       }
     };
-    if (bl.count > 0) load_k(0);
     for (int i = 0; i < bl.count; ++i) {
       if (i + 1 < bl.count) load_k(i + 1);
       const int k0 = bl.block(i) * kWaTile;
@@ -549,7 +549,7 @@ static bool wa_mappable(const void* base, const int64_t* st, int64_t B, int64_t 
 }
 
 bool window_sm100_takes(const mt_window_attention_desc& d) {
-  return d.dtype != MT_F32 && d.D <= 128 && d.scale > 0 && d.Sk > 0 && d.B * d.H <= 65535 &&
+  return d.dtype != MT_F32 && d.D <= 128 && d.scale > 0 && d.Sk > 0 && d.B * d.H <= INT32_MAX &&
          wa_mappable(d.q, d.q_strides, d.B, d.H, d.Sq, d.D) && wa_mappable(d.k, d.k_strides, d.B, d.Hkv, d.Sk, d.D) &&
          wa_mappable(d.v, d.v_strides, d.B, d.Hkv, d.Sk, d.D);
 }
@@ -575,7 +575,9 @@ static int wa_launch(const mt_window_attention_desc& d, const AttnParams& a, cud
   p.a = a;
   p.out_vec = d.o_strides[3] == 1 && (uintptr_t)d.o % 16 == 0 && d.o_strides[0] % 8 == 0 && d.o_strides[1] % 8 == 0 &&
               d.o_strides[2] % 8 == 0;
-  dim3 grid((unsigned)((d.Sq + 2 * kWaTile - 1) / (2 * kWaTile)), (unsigned)(d.B * d.H));
+  const int64_t blocks = (d.Sq + 2 * kWaTile - 1) / (2 * kWaTile);
+  if (blocks > 65535) return fail(MT_ERR_UNSUPPORTED, "window_attention: too many queries");
+  dim3 grid((unsigned)(d.B * d.H), (unsigned)blocks);
   kern<<<grid, kWaThreads, WaCfg<DP>::SMEM, st>>>(mq, mk, mv, p);
   return check_launch("window_attention_sm100");
 }
