@@ -8,7 +8,19 @@
 
 namespace mt {
 
+// n / d for n < 2^31 by a multiplication (d >= 1): m = floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div), s(0) {
+    while ((1ull << s) < div) ++s;
+    m = (uint32_t)((((1ull << s) - div) << 32) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
 struct Cache4Params {
+  FastDiv by_words, by_inner;  // D / 8; heads (append), tokens (read)
   const int32_t* table;
   int64_t table_stride;
   int max_pages, page_shift, num_pages;
@@ -57,8 +69,8 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p
   const uint32_t W = p.D / 8;
   const bool live = idx < (uint32_t)p.items;  // whole groups of 8 threads are live or not
   const uint32_t i = live ? idx : 0;
-  const uint32_t r = i / W, w = i - r * W;
-  const int t = r / (uint32_t)p.Hkv, h = r - (uint32_t)t * p.Hkv;
+  const uint32_t r = p.by_words.div(i), w = i - r * W;
+  const int t = p.by_inner.div(r), h = r - (uint32_t)t * p.Hkv;
   const int64_t row = live ? cache4_row(p, b, h, t) : -1;
   const T* src = static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
                  (int64_t)w * 8 * p.st[kv][3];
@@ -79,12 +91,30 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p
   const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
   const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
   const float z = __half2float(zero), s = __half2float(scale);
+  // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22 of
+  // itself of the divided one, so it rounds to the same code unless it is that near to a tie (within 2^-18 up to
+  // 15.5); then the words' quotients are divided as the definition says.  1.5 * 2^23 added to a number rounds it to a
+  // whole one, which stands in the sum's low bits.
+  constexpr float kRound = 12582912.f;
   uint32_t word = 0;
+  if (s > 0.f) {
+    const float inv = 1.f / s;
+    bool near = false;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    // the division is the definition's own rounding; rint ties go to the even code
-    const float c = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f) : 0.f;
-    word |= (uint32_t)c << (4 * j);
+    for (int j = 0; j < 8; ++j) {
+      const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inv), 0.f), 15.f);
+      const float r = __fadd_rn(q, kRound);
+      near |= fabsf(q - (r - kRound)) > 0.5f - 3.8e-6f;
+      word |= (__float_as_uint(r) & 15u) << (4 * j);
+    }
+    if (near) {
+      word = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
+        word |= (uint32_t)c << (4 * j);
+      }
+    }
   }
   p.words[kv][row * W + w] = (int32_t)word;
   if ((w & 7) == 0) p.scales[kv][row * (p.D / 64) + (w >> 3)] = __halves2half2(scale, zero);
@@ -97,8 +127,8 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) 
   const int64_t b = blockIdx.y >> 1;
   if (idx >= (uint32_t)p.items) return;
   const uint32_t W = p.D / 8;
-  const uint32_t r = idx / W, w = idx - r * W;
-  const int h = r / (uint32_t)p.T, t = r - (uint32_t)h * p.T;
+  const uint32_t r = p.by_words.div(idx), w = idx - r * W;
+  const int h = p.by_inner.div(r), t = r - (uint32_t)h * p.T;
   const int64_t row = cache4_row(p, b, h, t);
   uint32_t word = 0;
   float s = 0.f, z = 0.f;
@@ -112,7 +142,8 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) 
            (int64_t)w * 8 * p.st[kv][3];
   alignas(16) T v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(fmaf((float)((word >> (4 * j)) & 15u), s, z));
+  for (int j = 0; j < 8; ++j)  // 2^23 | code as a number, minus 2^23: the code
+    v[j] = from_f32<T>(fmaf(__uint_as_float(0x4b000000u | ((word >> (4 * j)) & 15u)) - 8388608.f, s, z));
   if (p.vec) {
 #pragma unroll
     for (int j = 0; j < (int)sizeof(T) / 2; ++j)
@@ -155,6 +186,7 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   if (B > 32767 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
   p.items = (int)(T * c.Hkv * (c.D / 8));
   p.starts = starts;
+  p.by_words = FastDiv((uint32_t)(c.D / 8));
   p.words[0] = c.k_words; p.words[1] = c.v_words;
   p.scales[0] = static_cast<__half2*>(c.k_scales); p.scales[1] = static_cast<__half2*>(c.v_scales);
   const int es = dtype_size(dtype);
@@ -175,6 +207,7 @@ int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_append");
   if (rc || B == 0 || p.items == 0) return rc;
   p.in[0] = k; p.in[1] = v;
+  p.by_inner = FastDiv((uint32_t)c.Hkv);
   dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
   switch (dtype) {
     case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
@@ -191,6 +224,7 @@ int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* 
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_read");
   if (rc || B == 0 || p.items == 0) return rc;
   p.out[0] = k; p.out[1] = v;
+  p.by_inner = FastDiv((uint32_t)T);
   dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
   switch (dtype) {
     case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;

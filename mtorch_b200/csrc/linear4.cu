@@ -4,13 +4,14 @@
 // is stored at place (w % 4) * 4 + w / 4 (see mtorch_cuda.h).
 //
 // linear4_kernel: Y^T = W X^T on mma.m16n8k16 with the weight's rows on the 16-row side and up to 8 * NT rows of X
-// on the 8-column side.  Bound by reading W: a lane's 16 bytes are words t, t + 4, t + 8, t + 12 of a block of 128
-// columns, which are its fragments for 8 products of 16 columns; no shared memory stands between.  A code's
-// 4 bits at the low end of a 16-bit lane are the number c * 2^-133 in bf16 (c * 2^-24 in f16), a subnormal that mma
-// multiplies exactly, at bits 4..7 sixteen times that: one AND makes two operands, one shift serves half a word.  X
-// is scaled to match while it is loaded (bf16 by 2^64; channels at bits 4..7 by another 1/16).  The code's offset
-// is taken off with one more product per step, of a constant row of eights: the same fp32 rounding as the
-// others, so nothing is left of it but sum x (c - 8).  Per group of columns: y += scale (acc - acc8), in fp32.
+// on the 8-column side.  Bound by reading W, and next by unpacking it: a lane's 16 bytes are words t, t + 4, t + 8,
+// t + 12 of a block of 128 columns, which are its fragments for 8 products of 16 columns.  A code's 4 bits at the low
+// end of a 16-bit lane are the number c * 2^-133 in bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly,
+// at bits 4..7 sixteen times that: one AND makes two operands, one shift serves half a word.  X is laid out once
+// per CTA as operands in shared memory, scaled to match (bf16 by 2^64; channels at bits 4..7 by another 1/16), with
+// the sums of 8 x per row and group beside it, which take the codes' offset off: y += scale (acc - sum 8 x), in fp32
+// per group of columns.  A warp brings its blocks of W with its own cp.async into a ring; no barrier stands between
+// the warps but at the end of a tile.
 //
 // fp32 X goes as three bf16 parts (8 + 8 + 8 bits) in three rows of their own, added at the end.
 #include <algorithm>
@@ -46,82 +47,203 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int kW4Warps = 8;
+// the same on sums of zero
+template <bool F16>
+__device__ __forceinline__ void w4_mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 
 // Rows of the products that one row of X becomes.
 template <typename T> constexpr int w4_parts() { return sizeof(T) == 4 ? 3 : 1; }
 
-// Eight columns of X at k as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7), scaled as the codes' places ask.
-// `part`: which of the three bf16 parts of fp32.
+// A code counts c * 2^-24 in f16, c * 2^-133 in bf16 against operands scaled by 2^64.
 template <typename T>
-__device__ __forceinline__ uint4 w4_load_x(const T* x, int k, int K, bool vec, int part) {
-  float v[8];
-  if (vec && k + 8 <= K) {
-    uint4 raw[sizeof(T) / 2];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(x + k) + i);
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f32<T>(x[k + j]) : 0.f;
-  }
-  constexpr bool F16 = std::is_same<T, __half>::value;
-  if (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float hi = __bfloat162float(__float2bfloat16_rn(v[j]));
-      const float mid = __bfloat162float(__float2bfloat16_rn(v[j] - hi));
-      v[j] = part == 0 ? hi : part == 1 ? mid : v[j] - hi - mid;
-    }
-  }
-  constexpr float even = F16 ? 1.f : 18446744073709551616.f, odd = even / 16.f;  // 2^64, 2^60
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float f = j & 1 ? odd : even;
-    w[j] = F16 ? pack_f16x2(v[j] * f, v[j + 4] * f) : pack_bf16x2(v[j] * f, v[j + 4] * f);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ constexpr float w4_unit() {
+  return std::is_same<T, __half>::value ? 16777216.f : 590295810358705651712.f;  // 2^24, 2^69
 }
 
-// One CTA: 16 * MT rows of W (outputs) against 8 * NT rows of operands; the 8 warps take blocks of 128 columns in
-// turn and add up in shared memory.
-template <typename T, int GROUP, int MT, int NT>
-__global__ void __launch_bounds__(kW4Warps * 32, MT * NT < 4 ? 2 : 1) linear4_kernel(const Linear4Params p) {
+// Eight columns of X as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7), scaled as the codes' places ask; bf16 exactly,
+// f16 but for what a sixteenth of values below 2^-10 loses (at most 2^-21).  `part`: which of the three bf16 parts of
+// fp32.  Returns 8 times the columns' sum in the operands' unit.
+template <typename T>
+__device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], int part, uint4& out) {
+  constexpr bool F16 = std::is_same<T, __half>::value;
+  const T* e = reinterpret_cast<const T*>(raw);
+  float sum = 0.f;
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 2) {
+    const uint4 r = raw[0];
+    w[0] = __byte_perm(r.x, r.z, 0x5410);
+    w[1] = __byte_perm(r.x, r.z, 0x7632);
+    w[2] = __byte_perm(r.y, r.w, 0x5410);
+    w[3] = __byte_perm(r.y, r.w, 0x7632);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (F16) {
+        __half2& v = *reinterpret_cast<__half2*>(&w[j]);
+        if (j & 1) v = __hmul2(v, __half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00)));  // 1/16
+      } else {
+        __nv_bfloat162& v = *reinterpret_cast<__nv_bfloat162*>(&w[j]);
+        const __nv_bfloat16 f = __ushort_as_bfloat16(j & 1 ? 0x5d80 : 0x5f80);  // 2^60, 2^64
+        v = __hmul2(v, __nv_bfloat162(f, f));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += to_f32<T>(e[j]);
+  } else {
+    constexpr float even = 18446744073709551616.f, odd = even / 16.f;  // 2^64, 2^60
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = to_f32<T>(e[j]);
+      const float hi = __bfloat162float(__float2bfloat16_rn(x));
+      const float mid = __bfloat162float(__float2bfloat16_rn(x - hi));
+      v[j] = __bfloat162float(__float2bfloat16_rn(part == 0 ? hi : part == 1 ? mid : x - hi - mid));
+      sum += v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(v[j] * (j & 1 ? odd : even), v[j + 4] * (j & 1 ? odd : even));
+  }
+  out = make_uint4(w[0], w[1], w[2], w[3]);
+  return sum * (8.f / w4_unit<T>());
+}
+
+// 16 bytes to shared memory
+__device__ __forceinline__ void w4_cp_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Shared memory of a CTA for `rows` operand rows: the warps' sums, the rings, X's operands, the sums of 8 x.
+template <int GROUP, int MT, int NT, int WARPS>
+struct W4Smem {
+  static constexpr int STAGES = 3;
+  static constexpr int RING = STAGES * MT * 1024;  // a warp's: 16 MT rows of 64 bytes a block
+  static __host__ __device__ int pitch(int Kp) { return Kp * 2 + 64; }  // of an operand row: two rows meet no bank twice
+  static __host__ __device__ int red(int rows) { return 2 * WARPS * rows * (16 * MT + 4) * 4; }
+  static __host__ __device__ int ops(int rows, int Kp) { return rows * pitch(Kp); }
+  static __host__ __device__ int sums(int Kp) { return Kp / GROUP * 8 * NT * 4; }
+  static __host__ __device__ int total(int rows, int Kp) { return red(rows) + WARPS * RING + ops(rows, Kp) + sums(Kp); }
+};
+
+// A CTA takes a run of strips of 16 rows of W (outputs), the same number for all but a strip, and goes through them MT at
+// a time against up to 8 * NT operand rows; its warps take blocks of 128 columns in turn and add up in shared memory.
+// The rings run on across the tiles: the next tile's first blocks come while this one is finished.
+template <typename T, int GROUP, int MT, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Params p) {
   constexpr bool F16 = std::is_same<T, __half>::value;
   constexpr int PARTS = w4_parts<T>();
   constexpr int GPB = 128 / GROUP;  // groups of a block
-  constexpr int OUT = 16 * MT, COL = 8 * NT;
-  __shared__ float red[kW4Warps][COL][OUT + 4];
+  constexpr int OUT = 16 * MT;
+  using Smem = W4Smem<GROUP, MT, NT, WARPS>;
+  extern __shared__ __align__(16) uint8_t w4_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * OUT, row0 = blockIdx.y * COL;
-  const int rows = p.M * PARTS;
-  const int blocks = p.Kp / 128;
+  const int blocks = p.Kp / 128, rows = p.M * PARTS;
+  float* red = reinterpret_cast<float*>(w4_smem);  // [2][WARPS][rows][OUT + 4]
+  uint8_t* ring = w4_smem + Smem::red(rows) + warp * Smem::RING;
+  uint8_t* ops = w4_smem + Smem::red(rows) + WARPS * Smem::RING;
+  float* sums = reinterpret_cast<float*>(ops + Smem::ops(rows, p.Kp));  // [group][8 NT]
+  const uint32_t ring_u32 = smem_u32(ring);
+  const int pitch_x = Smem::pitch(p.Kp);
+  const int strips = (p.N + 15) / 16;
+  const int s0 = (int)((int64_t)strips * blockIdx.x / gridDim.x), s1 = (int)((int64_t)strips * (blockIdx.x + 1) / gridDim.x);
+  const int last_row = min(p.N, s1 * 16) - 1;
 
-  const T* xrow[NT];
-  int part[NT];
-  bool live[NT];
+  // step q of this warp: block (q % per_tile) * WARPS + warp of the tile at strip s0 + q / per_tile * MT
+  const int per_tile = (blocks + WARPS - 1) / WARPS;
+  // the next step to bring: chunk t of rows n + 8 i (rows past the CTA's repeat its last)
+  const int64_t pitch = p.Kp / 2;
+  const uint8_t* wsrc[2 * MT];
+  int ln0 = s0 * 16, lkb = warp, lq = 0;
+  auto start_tile = [&]() {
 #pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    const int r = row0 + 8 * x + n;
-    live[x] = r < rows;
-    part[x] = r % PARTS;
-    xrow[x] = static_cast<const T*>(p.x) + (int64_t)(live[x] ? r / PARTS : 0) * p.ldx;
-  }
-  // rows n and n + 8 of each tile of W; rows past N repeat the last
-  const uint4* wrow[MT][2];
-  const __nv_bfloat16* srow[MT][2];
+    for (int i = 0; i < 2 * MT; ++i)
+      wsrc[i] = reinterpret_cast<const uint8_t*>(p.words) + min(ln0 + 8 * i + n, last_row) * pitch + warp * 64 + t * 16;
+  };
+  start_tile();
+  auto load = [&](int stage) {
+    if (ln0 <= last_row && lkb < blocks) {
+      const uint32_t dst = ring_u32 + stage * (MT * 1024) + lane * 16;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t r = min(n0 + 16 * i + n + 8 * h, p.N - 1);
-      wrow[i][h] = reinterpret_cast<const uint4*>(p.words + r * (p.Kp / 8)) + t;
-      srow[i][h] = p.scales + r * (p.Kp / GROUP);
+      for (int i = 0; i < 2 * MT; ++i) w4_cp_async(dst + i * 512, wsrc[i]);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    lkb += WARPS;
+    if (++lq == per_tile) {
+      lq = 0;
+      lkb = warp;
+      ln0 += OUT;
+      start_tile();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) wsrc[i] += WARPS * 64;
+    }
+  };
+  uint2 sc = make_uint2(0, 0);  // scales of row `lane` of the tile in the next block, as they come
+  const __nv_bfloat16* srow;
+  auto scales_of = [&](int n0) {
+    srow = p.scales + (int64_t)min(n0 + (lane & (OUT - 1)), last_row) * (p.Kp / GROUP);
+  };
+  auto load_scales = [&](int kb) {
+    if (kb >= blocks) return;
+    const __nv_bfloat16* s = srow + kb * GPB;
+    if (GPB == 4) sc = __ldg(reinterpret_cast<const uint2*>(s));
+    else if (GPB == 2) sc.x = __ldg(reinterpret_cast<const uint32_t*>(s));
+    else sc.x = __ldg(reinterpret_cast<const uint16_t*>(s));
+  };
+#pragma unroll
+  for (int s = 0; s < Smem::STAGES - 1; ++s) load(s);
+  scales_of(s0 * 16);
+  load_scales(warp);
 
+  // X's operands: a warp takes 32 chunks of 8 columns of a row at a time (a group's chunks are neighbouring lanes)
+  const int chunks = p.Kp / 8, segs = (chunks + 31) / 32, tasks = rows * segs;
+  constexpr int U = 4;  // loads in flight
+  for (int task0 = warp; task0 < tasks; task0 += U * WARPS) {
+    uint4 raw[U][sizeof(T) / 2];
+    int row[U], ch[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int task = min(task0 + u * WARPS, tasks - 1);
+      row[u] = task / segs;
+      ch[u] = (task - row[u] * segs) * 32 + lane;
+      const int k = ch[u] * 8;
+      const T* src = static_cast<const T*>(p.x) + (int64_t)(row[u] / PARTS) * p.ldx + k;
+      if (p.x_vec && k + 8 <= p.K) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[u][i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      } else {
+        T* e = reinterpret_cast<T*>(raw[u]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = k + j < p.K ? src[j] : from_f32<T>(0.f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint4 o;
+      float sum = w4_operands<T>(raw[u], row[u] % PARTS, o);
+#pragma unroll
+      for (int d = 1; d < GROUP / 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (task0 + u * WARPS < tasks && ch[u] < chunks) {
+        *reinterpret_cast<uint4*>(ops + row[u] * pitch_x + ch[u] * 16) = o;
+        if (ch[u] % (GROUP / 8) == 0) sums[ch[u] / (GROUP / 8) * (8 * NT) + row[u]] = sum;
+      }
+    }
+  }
+  __syncthreads();
+
+  const uint8_t* xrow[NT];  // this lane's operand rows (rows past the last repeat it; their sums are not stored)
+#pragma unroll
+  for (int x = 0; x < NT; ++x) xrow[x] = ops + min(8 * x + n, rows - 1) * pitch_x + t * 16;
   float y[MT][NT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -129,99 +251,109 @@ __global__ void __launch_bounds__(kW4Warps * 32, MT * NT < 4 ? 2 : 1) linear4_ke
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[i][x][e] = 0.f;
-
-  uint4 w[MT][2];
-  __nv_bfloat16 sc[MT][2][GPB];
-  auto load_w = [&](int kb) {
+  int stage = 0, buf = 0, q = 0, kb = warp;
+  for (int n0 = s0 * 16; n0 <= last_row;) {
+    if (kb < blocks) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Smem::STAGES - 2) : "memory");
+      __syncwarp();
+      const uint8_t* st = ring + stage * (MT * 1024) + lane * 16;
+      uint2 sn[MT][2];  // this block's scales; the next block's start to come
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        w[i][h] = __ldg(wrow[i][h] + kb * 4);
-        if (GPB == 4) *reinterpret_cast<uint2*>(sc[i][h]) = __ldg(reinterpret_cast<const uint2*>(srow[i][h] + kb * GPB));
-        else if (GPB == 2) *reinterpret_cast<uint32_t*>(sc[i][h]) = __ldg(reinterpret_cast<const uint32_t*>(srow[i][h] + kb * GPB));
-        else sc[i][h][0] = srow[i][h][kb];
+        for (int h = 0; h < 2; ++h) {
+          sn[i][h].x = __shfl_sync(0xffffffffu, sc.x, 16 * i + 8 * h + n);
+          sn[i][h].y = GPB == 4 ? __shfl_sync(0xffffffffu, sc.y, 16 * i + 8 * h + n) : 0u;
+        }
+      if (q + 1 < per_tile) load_scales(kb + WARPS);
+      uint4 xb[4][NT];
+      float2 s8[GPB][NT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xb[j][x] = *reinterpret_cast<const uint4*>(xrow[x] + kb * 256 + j * 64);
+#pragma unroll
+        for (int g = 0; g < GPB; ++g)
+          s8[g][x] = *reinterpret_cast<const float2*>(sums + (kb * GPB + g) * (8 * NT) + 8 * x + 2 * t);
       }
-  };
-  if (warp < blocks) load_w(warp);
-  for (int kb = warp; kb < blocks; kb += kW4Warps) {
-    uint4 wc[MT][2];
-    float sf[MT][2][GPB];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
+        const uint4 c0 = *reinterpret_cast<const uint4*>(st + i * 1024), c1 = *reinterpret_cast<const uint4*>(st + i * 1024 + 512);
+        float acc[NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        wc[i][h] = w[i][h];
+        for (int j = 0; j < 4; ++j) {  // 32 columns
+          const bool fresh = (j * 32) % GROUP == 0;
+          uint32_t w0 = j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w;
+          uint32_t w1 = j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w;
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) sf[i][h][g] = __bfloat162float(sc[i][h][g]);
-      }
-    if (kb + kW4Warps < blocks) load_w(kb + kW4Warps);
-    float acc[MT][NT][4], acc8[NT][4];
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // 32 columns
-      if ((j * 32) % GROUP == 0) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc8[x][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][x][e] = 0.f;
-          }
-      }
-      uint4 xb[NT];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-        xb[x] = live[x] ? w4_load_x<T>(xrow[x], kb * 128 + j * 32 + t * 8, p.K, p.x_vec, part[x]) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t eights[4] = {0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u};
-#pragma unroll
-        for (int x = 0; x < NT; ++x) w4_mma<F16>(acc8[x], eights, e ? xb[x].z : xb[x].x, e ? xb[x].w : xb[x].y);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint32_t w0 = j == 0 ? wc[i][0].x : j == 1 ? wc[i][0].y : j == 2 ? wc[i][0].z : wc[i][0].w;
-          uint32_t w1 = j == 0 ? wc[i][1].x : j == 1 ? wc[i][1].y : j == 2 ? wc[i][1].z : wc[i][1].w;
-          if (e) {
+            for (int x = 0; x < NT; ++x) {
+              if (fresh && e == 0) w4_mma_zero<F16>(acc[x], a, xb[j][x].x, xb[j][x].y);
+              else w4_mma<F16>(acc[x], a, e ? xb[j][x].z : xb[j][x].x, e ? xb[j][x].w : xb[j][x].y);
+            }
             w0 >>= 8;
             w1 >>= 8;
           }
-          const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+          if ((j * 32 + 32) % GROUP == 0) {
+            const int g = j * 32 / GROUP;
 #pragma unroll
-          for (int x = 0; x < NT; ++x) w4_mma<F16>(acc[i][x], a, e ? xb[x].z : xb[x].x, e ? xb[x].w : xb[x].y);
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = g < 2 ? sn[i][h].x : sn[i][h].y;
+              const float s = __uint_as_float(g & 1 ? w & 0xffff0000u : w << 16);
+#pragma unroll
+              for (int x = 0; x < NT; ++x) {
+                y[i][x][2 * h] = fmaf(s, acc[x][2 * h] - s8[g][x].x, y[i][x][2 * h]);
+                y[i][x][2 * h + 1] = fmaf(s, acc[x][2 * h + 1] - s8[g][x].y, y[i][x][2 * h + 1]);
+              }
+            }
+          }
         }
       }
-      if ((j * 32 + 32) % GROUP == 0) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              y[i][x][e] = fmaf(sf[i][e >> 1][j * 32 / GROUP], acc[i][x][e] - acc8[x][e], y[i][x][e]);
-      }
     }
+    if (q + 1 == per_tile) {
+      scales_of(n0 + OUT);
+      load_scales(warp);
+    }
+    __syncwarp();
+    int next = stage + Smem::STAGES - 1;
+    if (next >= Smem::STAGES) next -= Smem::STAGES;
+    load(next);
+    if (++stage == Smem::STAGES) stage = 0;
+    kb += WARPS;
+    if (++q < per_tile) continue;
+    // the tile is done: add the warps' sums (two buffers, so that one barrier a tile is enough)
+    float* mine = red + (buf * WARPS + warp) * rows * (OUT + 4);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 8 * x + 2 * t + (e & 1);
+          if (r < rows) mine[r * (OUT + 4) + 16 * i + n + 8 * (e >> 1)] = y[i][x][e];
+          y[i][x][e] = 0.f;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.M * OUT; i += WARPS * 32) {
+      const int m = i / OUT, c = i % OUT;
+      if (n0 + c > last_row) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) v += red[((buf * WARPS + k) * rows + m * PARTS + part) * (OUT + 4) + c];
+      v *= w4_unit<T>();
+      if (p.bias) v += to_f32<T>(static_cast<const T*>(p.bias)[n0 + c]);
+      static_cast<T*>(p.y)[(int64_t)m * p.ldy + n0 + c] = from_f32<T>(v);
+    }
+    buf ^= 1;
+    n0 += OUT;
+    q = 0;
+    kb = warp;
   }
-  constexpr float unit = F16 ? 16777216.f : 590295810358705651712.f;  // 2^24, 2^69
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][8 * x + 2 * t + (e & 1)][16 * i + n + 8 * (e >> 1)] = y[i][x][e] * unit;
-  __syncthreads();
-  const int m0 = row0 / PARTS, ms = min(COL / PARTS, p.M - m0);
-  for (int i = threadIdx.x; i < ms * OUT; i += kW4Warps * 32) {
-    const int m = i / OUT, c = i % OUT;
-    if (n0 + c >= p.N) continue;
-    float v = 0.f;
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q)
-#pragma unroll
-      for (int k = 0; k < kW4Warps; ++k) v += red[k][m * PARTS + q][c];
-    if (p.bias) v += to_f32<T>(static_cast<const T*>(p.bias)[n0 + c]);
-    static_cast<T*>(p.y)[(int64_t)(m0 + m) * p.ldy + n0 + c] = from_f32<T>(v);
-  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // One thread per word of 8 columns; the group's maximum over 4, 8 or 16 neighbouring threads.
@@ -290,50 +422,70 @@ static int w4_check(int64_t N, int64_t K, int64_t group, int dtype, const char* 
   return MT_OK;
 }
 
-// Rows of X that go through linear4_kernel; more go through an unpacked copy of W and the tensor-core GEMM.
-constexpr int64_t kW4MaxRows = 64;
+// Rows and columns of X that go through linear4_kernel (the operands of one row, three for fp32, have to fit the shared
+// memory); others go through an unpacked copy of W and the tensor-core GEMM.
+constexpr int64_t kW4MaxRows = 64, kW4MaxCols = 16384;
+static bool w4_few(const mt_linear_weight4_desc& d) { return d.M <= kW4MaxRows && d.K <= kW4MaxCols; }
 
-template <typename T, int GROUP, int MT, int NT>
-static void linear4_launch(const Linear4Params& p, cudaStream_t st) {
-  constexpr int per = 8 * NT / w4_parts<T>();  // rows of X a tile
-  Linear4Params q = p;
-  dim3 grid((unsigned)((p.N + 16 * MT - 1) / (16 * MT)), 1);
-  // fp32: 8 NT operand rows hold (8 NT / 3) whole rows of X
-  for (int m = 0; m < p.M; m += per) {
-    q.x = static_cast<const T*>(p.x) + (int64_t)m * p.ldx;
-    q.y = static_cast<T*>(p.y) + (int64_t)m * p.ldy;
-    q.M = std::min(per, p.M - m);
-    linear4_kernel<T, GROUP, MT, NT><<<grid, kW4Warps * 32, 0, st>>>(q);
-  }
+constexpr int kW4Smem = 227 * 1024;
+
+// Operand rows that fit a CTA of this shape.
+template <int GROUP, int MT, int NT, int WARPS>
+static int w4_fit(int Kp) {
+  using Smem = W4Smem<GROUP, MT, NT, WARPS>;
+  const int left = kW4Smem - Smem::total(0, Kp);
+  return left <= 0 ? 0 : std::min(8 * NT, left / (Smem::red(1) + Smem::ops(1, Kp)));
 }
 
-template <typename T, int GROUP>
-static void linear4_dispatch(const Linear4Params& p, cudaStream_t st) {
-  const int rows = p.M * w4_parts<T>();
-  // 64 rows of W a CTA where that still gives every SM two CTAs: X's operands are then made once for four tiles
-  bool wide = p.N >= 64 * 2 * num_sms(), mid = p.N >= 32 * 2 * num_sms();
-  if (getenv("MT_W4")) { int v = atoi(getenv("MT_W4")); wide = v == 4; mid = v >= 2; }
-  if (rows <= 8) {
-    if (wide) linear4_launch<T, GROUP, 4, 1>(p, st);
-    else if (mid) linear4_launch<T, GROUP, 2, 1>(p, st);
-    else linear4_launch<T, GROUP, 1, 1>(p, st);
-  } else if (rows <= 16) {
-    if (mid) linear4_launch<T, GROUP, 2, 2>(p, st);
-    else linear4_launch<T, GROUP, 1, 2>(p, st);
-  } else {
-    if (mid) linear4_launch<T, GROUP, 2, 4>(p, st);
-    else linear4_launch<T, GROUP, 1, 4>(p, st);
+template <typename T, int GROUP, int MT, int NT, int WARPS>
+static int linear4_launch(const Linear4Params& p, int rows_x, cudaStream_t st) {
+  auto kern = linear4_kernel<T, GROUP, MT, NT, WARPS>;
+  static bool attr[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem), "linear4 smem attribute");
+    if (rc) return rc;
+    attr[dev & 63] = true;
   }
+  Linear4Params q = p;
+  const int strips = (p.N + 15) / 16;
+  const unsigned grid = (unsigned)std::min((strips + MT - 1) / MT, num_sms());
+  for (int m = 0; m < p.M; m += rows_x) {
+    q.x = static_cast<const T*>(p.x) + (int64_t)m * p.ldx;
+    q.y = static_cast<T*>(p.y) + (int64_t)m * p.ldy;
+    q.M = std::min(rows_x, p.M - m);
+    kern<<<grid, WARPS * 32, W4Smem<GROUP, MT, NT, WARPS>::total(q.M * w4_parts<T>(), p.Kp), st>>>(q);
+    int rc = check_launch("linear_weight4");
+    if (rc) return rc;
+  }
+  return MT_OK;
+}
+
+// Rows of X a launch: as many as fit the shared memory, evenly over the launches.  One strip at a time but where every SM
+// has two and the registers allow it (up to 8 operand rows): X's operands are then read once for both.
+template <typename T, int GROUP>
+static int linear4_dispatch(const Linear4Params& p, cudaStream_t st) {
+  constexpr int PARTS = w4_parts<T>();
+  const bool two = p.N > 16 * num_sms();
+  const int fit1 = (two ? w4_fit<GROUP, 2, 1, 16>(p.Kp) : w4_fit<GROUP, 1, 1, 16>(p.Kp)) / PARTS;
+  const int fit2 = w4_fit<GROUP, 1, 2, 16>(p.Kp) / PARTS, fit4 = w4_fit<GROUP, 1, 4, 8>(p.Kp) / PARTS;
+  const int most = std::max(fit1, std::max(fit2, fit4));
+  if (most < 1) return fail(MT_ERR_UNSUPPORTED, "linear_weight4: %d columns do not fit the shared memory", p.K);
+  const int launches = (p.M + most - 1) / most, rows = (p.M + launches - 1) / launches;
+  if (rows <= fit1)
+    return two ? linear4_launch<T, GROUP, 2, 1, 16>(p, rows, st) : linear4_launch<T, GROUP, 1, 1, 16>(p, rows, st);
+  if (rows <= fit2) return linear4_launch<T, GROUP, 1, 2, 16>(p, rows, st);
+  return linear4_launch<T, GROUP, 1, 4, 8>(p, rows, st);
 }
 
 template <typename T>
 static int linear4_run(const Linear4Params& p, cudaStream_t st) {
   switch (p.group) {
-    case 32: linear4_dispatch<T, 32>(p, st); break;
-    case 64: linear4_dispatch<T, 64>(p, st); break;
-    default: linear4_dispatch<T, 128>(p, st);
+    case 32: return linear4_dispatch<T, 32>(p, st);
+    case 64: return linear4_dispatch<T, 64>(p, st);
+    default: return linear4_dispatch<T, 128>(p, st);
   }
-  return check_launch("linear_weight4");
 }
 
 static int validate_linear4(const mt_linear_weight4_desc& d) {
@@ -366,14 +518,14 @@ static size_t w4_copy_bytes(const mt_linear_weight4_desc& d) {
 }
 
 size_t linear_weight4_workspace(const mt_linear_weight4_desc& d) {
-  if (validate_linear4(d) || d.M <= kW4MaxRows || d.N == 0 || d.K == 0) return 0;
+  if (validate_linear4(d) || w4_few(d) || d.N == 0 || d.K == 0) return 0;
   return w4_copy_bytes(d) + gemm_workspace(w4_gemm(d, reinterpret_cast<void*>(1024)));
 }
 
 int run_linear_weight4(const mt_linear_weight4_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
   int rc = validate_linear4(d);
   if (rc || d.M == 0 || d.N == 0) return rc;
-  if (d.M > kW4MaxRows && d.K > 0) {
+  if (!w4_few(d) && d.K > 0) {
     if (!ws || ws_bytes < linear_weight4_workspace(d)) return fail(MT_ERR_WORKSPACE, "linear_weight4: workspace too small");
     rc = run_weight4_unpack(ws, d.dtype, w4_pitch(d), d.words, d.scales, d.N, d.K, d.group, st);
     if (rc) return rc;
