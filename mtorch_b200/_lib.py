@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmtorch_cuda.so"
@@ -127,6 +128,33 @@ class LinearWeight4Desc(C.Structure):
     ]
 
 
+def packer(desc):
+    """`pack` of a descriptor's fields, nested and arrays flattened, to the bytes of the C struct (a quarter of
+    the time of filling the ctypes structure: a decoder's step makes a few calls of microseconds)."""
+    codes = {I64: "q", C.c_int: "i", VP: "P", C.c_double: "d", C.c_size_t: "N", C.c_float: "f"}
+
+    def fields(cls):
+        out = ""
+        for _, t in cls._fields_:
+            if isinstance(t, type) and issubclass(t, C.Structure):
+                out += fields(t)
+            elif isinstance(t, type) and issubclass(t, C.Array):
+                out += codes[t._type_] * t._length_
+            else:
+                out += codes[t]
+        return out
+
+    st = struct.Struct("@" + fields(desc))
+    assert st.size == C.sizeof(desc), (desc, st.size)
+    return st.pack
+
+
+pack_rotary = packer(RotaryDesc)
+pack_window_attention = packer(WindowAttentionDesc)
+pack_kv_cache4_attention = packer(KvCache4AttentionDesc)
+pack_linear_weight4 = packer(LinearWeight4Desc)
+
+
 class RngState(C.Structure):
     _fields_ = [("state", C.c_uint64), ("has_spare", C.c_int32), ("spare", C.c_double)]
 
@@ -203,17 +231,18 @@ SIGNATURES = {
     "mt_cuda_sdpa_workspace_size": (C.c_size_t, [C.POINTER(SdpaDesc)]),
     "mt_cuda_sdpa": (C.c_int, [C.POINTER(SdpaDesc), VP, C.c_size_t, VP]),
     "mt_cuda_sdpa_path": (C.c_int, [C.POINTER(SdpaDesc)]),
-    "mt_cuda_rotary": (C.c_int, [C.POINTER(RotaryDesc), VP]),
-    "mt_cuda_window_attention_workspace_size": (C.c_size_t, [C.POINTER(WindowAttentionDesc)]),
-    "mt_cuda_window_attention": (C.c_int, [C.POINTER(WindowAttentionDesc), VP, C.c_size_t, VP]),
+    # (descriptors as packed bytes or byref: `packer`)
+    "mt_cuda_rotary": (C.c_int, [VP, VP]),
+    "mt_cuda_window_attention_workspace_size": (C.c_size_t, [VP]),
+    "mt_cuda_window_attention": (C.c_int, [VP, VP, C.c_size_t, VP]),
     "mt_cuda_kv_cache4_append": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
                                            I64, VP, VP]),
     "mt_cuda_kv_cache4_read": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
                                          I64, VP, VP]),
-    "mt_cuda_kv_cache4_attention_workspace_size": (C.c_size_t, [C.POINTER(KvCache4AttentionDesc)]),
-    "mt_cuda_kv_cache4_attention": (C.c_int, [C.POINTER(KvCache4AttentionDesc), VP, C.c_size_t, VP]),
-    "mt_cuda_linear_weight4_workspace_size": (C.c_size_t, [C.POINTER(LinearWeight4Desc)]),
-    "mt_cuda_linear_weight4": (C.c_int, [C.POINTER(LinearWeight4Desc), VP, C.c_size_t, VP]),
+    "mt_cuda_kv_cache4_attention_workspace_size": (C.c_size_t, [VP]),
+    "mt_cuda_kv_cache4_attention": (C.c_int, [VP, VP, C.c_size_t, VP]),
+    "mt_cuda_linear_weight4_workspace_size": (C.c_size_t, [VP]),
+    "mt_cuda_linear_weight4": (C.c_int, [VP, VP, C.c_size_t, VP]),
     "mt_cuda_weight4_pack": (C.c_int, [VP, VP, VP, C.c_int, I64, I64, I64, I64, VP]),
     "mt_cuda_weight4_unpack": (C.c_int, [VP, C.c_int, I64, VP, VP, I64, I64, I64, VP]),
     "mt_rng_seed": (None, [C.POINTER(RngState), C.c_uint64]),

@@ -15,13 +15,33 @@ import numpy as np
 
 from . import _lib as L
 from .ops import _lib, _same_dtype
-from .tensor import (Tensor, _new, _require_cuda, bfloat16, device as _device, float16, float32, int32, tensor, to_dtype,
-                     workspace, zeros)
+from .tensor import (_WS, Tensor, _new, _require_cuda, bfloat16, device as _device, float16, float32, int32, stream_ptr,
+                     tensor, to_dtype, workspace, zeros)
 
 CACHE_GROUP = 64  # channels of a head that share a scale and a zero point in KVCache4
 
 
+# These calls take microseconds on the device, so what stands before them on the host is kept short: descriptors are
+# packed at once (L.packer) and the shared workspace is asked for only when it is too small.
+
+
 def _check(rc, what):
+    if rc:
+        L.check(rc, what)
+
+
+def _ptr(t):
+    return t._buf.ptr + t._offset * t.dtype.itemsize
+
+
+def _run(fn, size_fn, desc, t, what):
+    """fn(desc, workspace, its size, stream), with the device's workspace grown where it does not suffice."""
+    idx = t.device.index or 0
+    buf, stream = _WS.get(idx), stream_ptr(idx)
+    rc = fn(desc, buf.ptr, buf.nbytes, stream) if buf is not None else fn(desc, None, 0, stream)
+    if rc == L.MT_ERR_WORKSPACE:
+        ws, n = workspace(size_fn(desc), idx)
+        rc = fn(desc, ws, n, stream)
     if rc:
         L.check(rc, what)
 
@@ -40,9 +60,8 @@ def _check_out(out, shape, like, what):
         raise RuntimeError(f"{what}: out has shape {list(out._shape)}, expected {list(shape)}")
     if out.dtype is not like.dtype or out.device.type != "cuda":
         raise ValueError(f"{what}: out has to be a {like.dtype.name} tensor on the cuda device")
-    for n, s in zip(out._shape, out._strides):
-        if n > 1 and s == 0:
-            raise ValueError(f"{what}: out is an expanded view")
+    if 0 in out._strides and any(n > 1 and s == 0 for n, s in zip(out._shape, out._strides)):
+        raise ValueError(f"{what}: out is an expanded view")
     return out
 
 
@@ -97,7 +116,7 @@ def rotary_embedding(q: Tensor, k: Tensor | None, positions: Tensor, frequencies
         raise ValueError(f"{what}: positions have to be int32 [{axes}, {S}] or [{axes}, {B}, {S}]")
     if S > 1 and positions._strides[-1] != 1:
         positions = positions.contiguous()
-    if frequencies.dtype is not float32 or frequencies._shape != (pairs,) or not frequencies.is_contiguous():
+    if frequencies.dtype is not float32 or frequencies._shape != (pairs,) or (pairs > 1 and frequencies._strides != (1,)):
         raise ValueError(f"{what}: frequencies have to be float32 [{pairs}]")
     if out is None:
         oq = _new_heads(B, Hq, S, D, q)
@@ -115,12 +134,11 @@ def rotary_embedding(q: Tensor, k: Tensor | None, positions: Tensor, frequencies
         at += n
         ends[a] = at
     pb = positions._strides[1] if positions.dim() == 3 and positions._shape[1] > 1 else 0
-    d = L.RotaryDesc(B, S, D, Hq, k._shape[1] if k is not None else 0, q.dtype.code, bool(interleaved), bool(inverse),
-                     axes, pairs, tuple(ends), positions.data_ptr(), positions._strides[0], pb,
-                     frequencies.data_ptr(), q.data_ptr(), q._strides, oq.data_ptr(), oq._strides)
-    if k is not None:
-        d.k, d.k_strides, d.k_out, d.k_out_strides = k.data_ptr(), k._strides, ok.data_ptr(), ok._strides
-    _check(_lib().mt_cuda_rotary(C.byref(d), q._stream()), what)
+    kq = (_ptr(k), *k._strides, _ptr(ok), *ok._strides) if k is not None else (0,) * 10
+    d = L.pack_rotary(B, S, D, Hq, k._shape[1] if k is not None else 0, q.dtype.code, bool(interleaved), bool(inverse),
+                      axes, pairs, *ends, _ptr(positions), positions._strides[0], pb, _ptr(frequencies), _ptr(q),
+                      *q._strides, _ptr(oq), *oq._strides, *kq)
+    _check(_lib().mt_cuda_rotary(d, stream_ptr(q.device.index or 0)), what)
     oq._mark_modified()
     if k is None:
         return oq
@@ -170,15 +188,12 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int | None, sinks:
         out = _new_heads(B, H, Sq, D, q)
     else:
         _check_out(out, q._shape, q, what)
-    d = L.WindowAttentionDesc(
-        B, H, Hkv, Sq, Sk, D, q.dtype.code, bool(causal), w, int(sinks),
-        starts.data_ptr() if starts is not None else None, lengths.data_ptr() if lengths is not None else None,
-        q.data_ptr(), q._strides, k.data_ptr(), k._strides, v.data_ptr(), v._strides, out.data_ptr(), out._strides,
-        float(scale) if scale is not None else 1.0 / math.sqrt(D))
+    d = L.pack_window_attention(
+        B, H, Hkv, Sq, Sk, D, q.dtype.code, bool(causal), w, int(sinks), _ptr(starts) if starts is not None else 0,
+        _ptr(lengths) if lengths is not None else 0, _ptr(q), *q._strides, _ptr(k), *k._strides, _ptr(v), *v._strides,
+        _ptr(out), *out._strides, float(scale) if scale is not None else 1.0 / math.sqrt(D))
     lib = _lib()
-    ref = C.byref(d)
-    ws, wsb = workspace(lib.mt_cuda_window_attention_workspace_size(ref), q._idx())
-    _check(lib.mt_cuda_window_attention(ref, ws, wsb, q._stream()), what)
+    _run(lib.mt_cuda_window_attention, lib.mt_cuda_window_attention_workspace_size, d, q, what)
     out._mark_modified()
     return out
 
@@ -214,8 +229,9 @@ class KVCache4:
         self.k_words, self.k_scales, self.v_words, self.v_scales = k_words, k_scales, v_words, v_scales
         self.num_pages, self.heads, self.page_size, self.dim = pages, heads, page, w * 8
         self.device = k_words.device
-        self._desc = L.KvCache4Desc(pages, page, heads, w * 8, k_words.data_ptr(), k_scales.data_ptr(),
-                                    v_words.data_ptr(), v_scales.data_ptr())
+        self._fields = (pages, page, heads, w * 8, k_words.data_ptr(), k_scales.data_ptr(), v_words.data_ptr(),
+                        v_scales.data_ptr())
+        self._desc = C.byref(L.KvCache4Desc(*self._fields))
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, heads: int, dim: int, device="cuda") -> "KVCache4":
@@ -250,9 +266,8 @@ def _cache_move(cache, k, v, table, starts, T, fn, what):
                          f"and {list(v._shape)}")
     _check_table(cache, table, B, what)
     _require_int32(what, (B,), starts=starts)
-    _check(fn(C.byref(cache._desc), k.data_ptr(), (L.I64_4)(*k._strides), v.data_ptr(), (L.I64_4)(*v._strides),
-              k.dtype.code, B, T, table.data_ptr(), table._strides[0], table._shape[1], starts.data_ptr(),
-              cache.k_words._stream()), what)
+    _check(fn(cache._desc, _ptr(k), L.I64_4(*k._strides), _ptr(v), L.I64_4(*v._strides), k.dtype.code, B, T, _ptr(table),
+              table._strides[0], table._shape[1], _ptr(starts), stream_ptr(cache.device.index or 0)), what)
 
 
 def kv_cache_append(cache: KVCache4, k: Tensor, v: Tensor, block_table: Tensor, starts: Tensor) -> None:
@@ -311,14 +326,12 @@ def kv_cache_attention(q: Tensor, cache: KVCache4, block_table: Tensor, lengths:
         out = _new_heads(B, H, Sq, D, q)
     else:
         _check_out(out, q._shape, q, what)
-    d = L.KvCache4AttentionDesc(
-        cache._desc, B, H, Sq, q.dtype.code, w, int(sinks), block_table.data_ptr(), block_table._strides[0],
-        block_table._shape[1], lengths.data_ptr(), q.data_ptr(), q._strides, out.data_ptr(), out._strides,
+    d = L.pack_kv_cache4_attention(
+        *cache._fields, B, H, Sq, q.dtype.code, w, int(sinks), _ptr(block_table), block_table._strides[0],
+        block_table._shape[1], _ptr(lengths), _ptr(q), *q._strides, _ptr(out), *out._strides,
         float(scale) if scale is not None else 1.0 / math.sqrt(D))
     lib = _lib()
-    ref = C.byref(d)
-    ws, wsb = workspace(lib.mt_cuda_kv_cache4_attention_workspace_size(ref), q._idx())
-    _check(lib.mt_cuda_kv_cache4_attention(ref, ws, wsb, q._stream()), what)
+    _run(lib.mt_cuda_kv_cache4_attention, lib.mt_cuda_kv_cache4_attention_workspace_size, d, q, what)
     out._mark_modified()
     return out
 
@@ -401,12 +414,9 @@ def linear_weight4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, ou
         if weight.out > 1 and out._strides[-1] != 1 or (out.dim() != 2 and not out.is_contiguous()):
             raise ValueError(f"{what}: out has to have unit-stride rows")
         ldy = out._strides[0] if out.dim() == 2 else weight.out
-    d = L.LinearWeight4Desc(M, weight.out, weight.cols, weight.group, x.dtype.code, x.data_ptr(), x._strides[0],
-                            weight.words.data_ptr(), weight.scales.data_ptr(),
-                            bias.data_ptr() if bias is not None else None, out.data_ptr(), ldy)
+    d = L.pack_linear_weight4(M, weight.out, weight.cols, weight.group, x.dtype.code, _ptr(x), x._strides[0],
+                              _ptr(weight.words), _ptr(weight.scales), _ptr(bias) if bias is not None else 0, _ptr(out), ldy)
     lib = _lib()
-    ref = C.byref(d)
-    ws, wsb = workspace(lib.mt_cuda_linear_weight4_workspace_size(ref), x._idx())
-    _check(lib.mt_cuda_linear_weight4(ref, ws, wsb, x._stream()), what)
+    _run(lib.mt_cuda_linear_weight4, lib.mt_cuda_linear_weight4_workspace_size, d, x, what)
     out._mark_modified()
     return out
