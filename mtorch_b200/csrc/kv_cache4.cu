@@ -47,110 +47,122 @@ __device__ __forceinline__ int64_t cache4_row(const Cache4Params& p, int64_t b, 
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, int64_t st, bool vec, float (&x)[8]) {
+struct Vec8 {
+  alignas(16) T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8(const T* src, int64_t st, bool vec) {
+  Vec8<T> x;
   if (vec) {
-    uint4 raw[sizeof(T) / 2];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(src)[i];
-    const T* v = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(v[i]);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x.v)[i] = reinterpret_cast<const uint4*>(src)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[i * st]);
+    for (int i = 0; i < 8; ++i) x.v[i] = src[i * st];
   }
+  return x;
 }
 
+// A thread takes the same word of K and of V: one look into the table, two values' loads in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const int kv = blockIdx.y & 1;
-  const int64_t b = blockIdx.y >> 1;
+  const int64_t b = blockIdx.y;
   const uint32_t W = p.D / 8;
   const bool live = idx < (uint32_t)p.items;  // whole groups of 8 threads are live or not
   const uint32_t i = live ? idx : 0;
   const uint32_t r = p.by_words.div(i), w = i - r * W;
   const int t = p.by_inner.div(r), h = r - (uint32_t)t * p.Hkv;
+  Vec8<T> in[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+    in[kv] = load8<T>(static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
+                          (int64_t)w * 8 * p.st[kv][3], p.st[kv][3], p.vec);
   const int64_t row = live ? cache4_row(p, b, h, t) : -1;
-  const T* src = static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
-                 (int64_t)w * 8 * p.st[kv][3];
-  float x[8];
-  load8<T>(src, p.st[kv][3], p.vec, x);
-  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int j = 1; j < 8; ++j) {
-    lo = fminf(lo, x[j]);
-    hi = fmaxf(hi, x[j]);
-  }
+  for (int kv = 0; kv < 2; ++kv) {
+    float x[8];
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (row < 0) return;
-  const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
-  const float z = __half2float(zero), s = __half2float(scale);
-  // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22 of
-  // itself of the divided one, so it rounds to the same code unless it is that near to a tie (within 2^-18 up to
-  // 15.5); then the words' quotients are divided as the definition says.  1.5 * 2^23 added to a number rounds it to a
-  // whole one, which stands in the sum's low bits.
-  constexpr float kRound = 12582912.f;
-  uint32_t word = 0;
-  if (s > 0.f) {
-    const float inv = 1.f / s;
-    bool near = false;
+    for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(in[kv].v[j]);
+    float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inv), 0.f), 15.f);
-      const float r = __fadd_rn(q, kRound);
-      near |= fabsf(q - (r - kRound)) > 0.5f - 3.8e-6f;
-      word |= (__float_as_uint(r) & 15u) << (4 * j);
+    for (int j = 1; j < 8; ++j) {
+      lo = fminf(lo, x[j]);
+      hi = fmaxf(hi, x[j]);
     }
-    if (near) {
-      word = 0;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+    const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
+    const float z = __half2float(zero), s = __half2float(scale);
+    // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22
+    // of itself of the divided one, so it rounds to the same code unless it is that near to a tie (within 2^-18 up to
+    // 15.5); then the word's quotients are divided as the definition says.  1.5 * 2^23 added to a number rounds it to
+    // a whole one, which stands in the sum's low bits.
+    constexpr float kRound = 12582912.f;
+    uint32_t word = 0;
+    if (s > 0.f) {
+      const float inv = 1.f / s;
+      float tie = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
-        word |= (uint32_t)c << (4 * j);
+        const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inv), 0.f), 15.f);
+        const float r2 = __fadd_rn(q, kRound);
+        tie = fmaxf(tie, fabsf(q - (r2 - kRound)));
+        word |= (__float_as_uint(r2) & 15u) << (4 * j);
+      }
+      if (tie > 0.5f - 3.8e-6f) {
+        word = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
+          word |= (uint32_t)c << (4 * j);
+        }
       }
     }
+    if (row >= 0) {
+      p.words[kv][row * W + w] = (int32_t)word;
+      if ((w & 7) == 0) p.scales[kv][row * (W / 8) + (w >> 3)] = __halves2half2(scale, zero);
+    }
   }
-  p.words[kv][row * W + w] = (int32_t)word;
-  if ((w & 7) == 0) p.scales[kv][row * (p.D / 64) + (w >> 3)] = __halves2half2(scale, zero);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const int kv = blockIdx.y & 1;
-  const int64_t b = blockIdx.y >> 1;
+  const int64_t b = blockIdx.y;
   if (idx >= (uint32_t)p.items) return;
   const uint32_t W = p.D / 8;
   const uint32_t r = p.by_words.div(idx), w = idx - r * W;
   const int h = p.by_inner.div(r), t = r - (uint32_t)h * p.T;
   const int64_t row = cache4_row(p, b, h, t);
-  uint32_t word = 0;
-  float s = 0.f, z = 0.f;
+  uint32_t word[2] = {0, 0};
+  float2 sz[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   if (row >= 0) {
-    word = (uint32_t)p.words[kv][row * W + w];
-    const __half2 sz = p.scales[kv][row * (p.D / 64) + (w >> 3)];
-    s = __low2float(sz);
-    z = __high2float(sz);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      word[kv] = (uint32_t)p.words[kv][row * W + w];
+      sz[kv] = __half22float2(p.scales[kv][row * (W / 8) + (w >> 3)]);
+    }
   }
-  T* dst = static_cast<T*>(p.out[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
-           (int64_t)w * 8 * p.st[kv][3];
-  alignas(16) T v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)  // 2^23 | code as a number, minus 2^23: the code
-    v[j] = from_f32<T>(fmaf(__uint_as_float(0x4b000000u | ((word >> (4 * j)) & 15u)) - 8388608.f, s, z));
-  if (p.vec) {
+  for (int kv = 0; kv < 2; ++kv) {
+    T* dst = static_cast<T*>(p.out[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
+             (int64_t)w * 8 * p.st[kv][3];
+    Vec8<T> o;
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j)
-      reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(v)[j];
-  } else {
+    for (int j = 0; j < 8; ++j)  // 2^23 | code as a number, minus 2^23: the code
+      o.v[j] = from_f32<T>(fmaf(__uint_as_float(0x4b000000u | ((word[kv] >> (4 * j)) & 15u)) - 8388608.f, sz[kv].x, sz[kv].y));
+    if (p.vec) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dst[j * p.st[kv][3]] = v[j];
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(o.v)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dst[j * p.st[kv][3]] = o.v[j];
+    }
   }
 }
 
@@ -183,7 +195,7 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   p.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
   p.num_pages = (int)c.num_pages;
   p.Hkv = (int)c.Hkv; p.D = (int)c.D; p.T = (int)T;
-  if (B > 32767 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
+  if (B > 65535 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
   p.items = (int)(T * c.Hkv * (c.D / 8));
   p.starts = starts;
   p.by_words = FastDiv((uint32_t)(c.D / 8));
@@ -208,7 +220,7 @@ int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks
   if (rc || B == 0 || p.items == 0) return rc;
   p.in[0] = k; p.in[1] = v;
   p.by_inner = FastDiv((uint32_t)c.Hkv);
-  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
+  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)B);
   switch (dtype) {
     case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
     case MT_BF16: cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
@@ -225,7 +237,7 @@ int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* 
   if (rc || B == 0 || p.items == 0) return rc;
   p.out[0] = k; p.out[1] = v;
   p.by_inner = FastDiv((uint32_t)T);
-  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)(2 * B));
+  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)B);
   switch (dtype) {
     case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;
     case MT_BF16: cache4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;

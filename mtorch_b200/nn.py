@@ -12,7 +12,7 @@ import math
 from collections import OrderedDict
 
 from . import _lib as L
-from . import ops
+from . import decoding, ops
 from .tensor import Tensor, empty, float32, to_dtype, device as _device
 
 
@@ -360,6 +360,9 @@ class _Functional:
     relu = staticmethod(ops.relu)
     sigmoid = staticmethod(ops.sigmoid)
     embedding = staticmethod(ops.embedding)
+    rotary_embedding = staticmethod(decoding.rotary_embedding)
+    window_attention = staticmethod(decoding.window_attention)
+    linear_weight4 = staticmethod(decoding.linear_weight4)
 
     @staticmethod
     def interpolate(x, size=None, scale_factor=None, mode="nearest", align_corners=None):
