@@ -14,8 +14,8 @@
 // the products far from fp32's own subnormals, their channels at bits 4..7 by 2^60.  With value = zero + scale c:
 //   q.k = scale (q.c) + zero sum(q)  per 64 channels,
 //   o   = sum (p scale) c + sum p zero,
-// with p scale rounded to bf16 (for f16 queries too: p scale spans more than f16's exponents).  That
-// rounding meets c - 8 rather than c, because what is added for zero is p (zero + 8 scale) - 8 round(p scale):
+// with p scale rounded to bf16 (for f16 queries too, whose exponents are too few for p scale; they get the rounding's
+// rest in a second product).  That rounding meets c - 8 rather than c, because what is added for zero is p (zero + 8 scale) - 8 round(p scale):
 // the codes of a key centre around 8, and the error of a rounded weight is halved.
 //
 // The running maximum is raised only when a score passes it by more than 2^8 ("lazy"): then the warp
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      uint32_t pb[NT][2];
+      uint32_t pb[NT][2], pl[NT][2];  // weights, and what their rounding to bf16 left (f16 over the codes)
       if (!PAGED) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -496,12 +496,19 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
             for (int x = 0; x < NT; ++x) {
               cor[x][c][0] = fmaf(sc[kb][x][2 * h], z, cor[x][c][0]);
               cor[x][c][1] = fmaf(sc[kb][x][2 * h + 1], z, cor[x][c][1]);
-              pb[x][h] = transpose8x8(pack_bf16x2(sc[kb][x][2 * h] * f, sc[kb][x][2 * h + 1] * f));
+              const float e0 = sc[kb][x][2 * h] * f, e1 = sc[kb][x][2 * h + 1] * f;
+              const uint32_t w = pack_bf16x2(e0, e1);
+              pb[x][h] = transpose8x8(w);
+              if (F16)
+                pl[x][h] = transpose8x8(pack_bf16x2(e0 - __uint_as_float(w << 16), e1 - __uint_as_float(w & 0xffff0000u)));
             }
           }
           const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-          for (int x = 0; x < NT; ++x) mma16816<false>(psum[PAGED ? c : 0][x], ones, pb[x][0], pb[x][1]);
+          for (int x = 0; x < NT; ++x) {
+            mma16816<false>(psum[PAGED ? c : 0][x], ones, pb[x][0], pb[x][1]);
+            if (F16) mma16816<false>(psum[PAGED ? c : 0][x], ones, pl[x][0], pl[x][1]);
+          }
           uint32_t vq[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -515,7 +522,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
             const uint32_t a[4] = {code_pair(w0, w0 >> 8, q), code_pair(w0, w0 >> 8, q + 1), code_pair(w1, w1 >> 8, q),
                                    code_pair(w1, w1 >> 8, q + 1)};
 #pragma unroll
-            for (int x = 0; x < NT; ++x) mma16816<false>(o[c][j][x], a, pb[x][0], pb[x][1]);
+            for (int x = 0; x < NT; ++x) {
+              mma16816<false>(o[c][j][x], a, pb[x][0], pb[x][1]);
+              if (F16) mma16816<false>(o[c][j][x], a, pl[x][0], pl[x][1]);
+            }
           }
         } else {
           uint32_t e0[4], e1[4], e2[4], e3[4];
