@@ -419,6 +419,14 @@ typedef struct {
 size_t mt_cuda_window_attention_workspace_size(const mt_window_attention_desc* desc);
 int mt_cuda_window_attention(const mt_window_attention_desc* desc, void* workspace, size_t workspace_bytes,
                              void* stream);
+/* Which kernel mt_cuda_window_attention runs for `desc`: tcgen05 tiles (16-bit, mappable rows, D <= 128, scale > 0,
+ * many queries), split keys on mma (16-bit, 16-byte aligned rows), fp32 tiles (many queries) or rows with
+ * split keys.  0 for an invalid descriptor. */
+#define MT_WINDOW_PATH_TC 1
+#define MT_WINDOW_PATH_SPLIT 2
+#define MT_WINDOW_PATH_TILES 3
+#define MT_WINDOW_PATH_ROWS 4
+int mt_cuda_window_attention_path(const mt_window_attention_desc* desc);
 
 /*
  * A paged key / value cache held in 4 bits.  Four contiguous arrays:

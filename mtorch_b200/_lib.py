@@ -235,6 +235,7 @@ SIGNATURES = {
     "mt_cuda_rotary": (C.c_int, [VP, VP]),
     "mt_cuda_window_attention_workspace_size": (C.c_size_t, [VP]),
     "mt_cuda_window_attention": (C.c_int, [VP, VP, C.c_size_t, VP]),
+    "mt_cuda_window_attention_path": (C.c_int, [VP]),
     "mt_cuda_kv_cache4_append": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
                                            I64, VP, VP]),
     "mt_cuda_kv_cache4_read": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,

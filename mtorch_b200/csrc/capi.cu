@@ -337,6 +337,10 @@ int mt_cuda_window_attention(const mt_window_attention_desc* desc, void* workspa
   return run_window_attention(*desc, workspace, workspace_bytes, S(stream));
 }
 
+int mt_cuda_window_attention_path(const mt_window_attention_desc* desc) {
+  return desc ? window_attention_path(*desc) : 0;
+}
+
 int mt_cuda_kv_cache4_append(const mt_kv_cache4* cache, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
                              int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream) {

@@ -108,6 +108,7 @@ int sdpa_tc_path(const mt_sdpa_desc& d);
 int run_rotary(const mt_rotary_desc& d, cudaStream_t st);
 size_t window_attention_workspace(const mt_window_attention_desc& d);
 int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+int window_attention_path(const mt_window_attention_desc& d);
 int validate_kv_cache4(const mt_kv_cache4& c);
 int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
                          int dtype, int64_t B, int64_t T, const int32_t* table, int64_t table_stride,

@@ -7,6 +7,7 @@
 // idle, so their keys are split over CTAs; the partial (m, l, o) go to the workspace and are joined
 // by a second kernel.
 #include <algorithm>
+#include <cmath>
 
 #include "window_attention.cuh"
 
@@ -164,6 +165,152 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many queries in fp32 (and 16-bit rows that the tensor-core kernel cannot map): tiles of 64 queries of a head by 64
+// keys in shared memory, fp32 products on the FMA units.  A thread (ty, tx) of 16 x 16 holds 4 x 4 scores and
+// 4 x (DP / 16) outputs; Q, K and P lie transposed, so that a step of a product is two 16-byte reads for 16 FMAs.
+// Bound by the FMA units (128 a cycle and SM); a tile past the window, or past the sinks, is not visited.
+constexpr int kTile = 64;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_tile_kernel(const AttnParams p, const bool aligned) {
+  extern __shared__ float4 tile_smem[];
+  float* Qs = reinterpret_cast<float*>(tile_smem);  // [DP][64]
+  float* Ks = Qs + DP * kTile;                      // [DP][64]
+  float* Vs = Ks + DP * kTile;                      // [64][DP]
+  float* Ps = Vs + DP * kTile;                      // [64 keys][64 queries]
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, hk = h / p.g;
+  const int q0 = (gridDim.y - 1 - blockIdx.y) * kTile, q1 = min(p.Sq, q0 + kTile) - 1;  // (the longest rows first)
+  const SeqPos sp = seq_pos(p, b, false);
+  const BlockList bl = block_list<kTile>(p, sp, sp.start + q0, sp.start + q1);
+  const RowKeys ra = row_keys(p, sp, sp.start + q0), rz = row_keys(p, sp, sp.start + q1);
+
+  // four channels of row `row` of a tensor; zeros where there are none
+  auto load4 = [&](const void* base, const int64_t* st, int64_t head, int row, bool live, int d) -> float4 {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live && d < p.D) {
+      const T* src = static_cast<const T*>(base) + b * st[0] + head * st[1] + row * st[2];
+      if (aligned) {
+        alignas(16) T raw[4];
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + d);
+        else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = to_f32<T>(raw[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < p.D) x[j] = to_f32<T>(src[(d + j) * st[3]]);
+      }
+    }
+    return make_float4(x[0], x[1], x[2], x[3]);
+  };
+
+  for (int i = tid; i < kTile * (DP / 4); i += 256) {
+    const int r = i % kTile, d = i / kTile * 4;
+    const float4 x = load4(p.q, p.qs, h, q0 + r, q0 + r < p.Sq, d);
+    Qs[d * kTile + r] = x.x * p.scale_log2;
+    Qs[(d + 1) * kTile + r] = x.y * p.scale_log2;
+    Qs[(d + 2) * kTile + r] = x.z * p.scale_log2;
+    Qs[(d + 3) * kTile + r] = x.w * p.scale_log2;
+  }
+  float m[4], l[4], o[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) o[i][j] = 0.f;
+  }
+  for (int t = 0; t < bl.count; ++t) {
+    const int k0 = bl.block(t) * kTile;
+    __syncthreads();
+    for (int i = tid; i < kTile * (DP / 4); i += 256) {
+      const int r = i % kTile, d = i / kTile * 4;  // K: neighbouring threads take neighbouring keys
+      const float4 x = load4(p.k, p.ks, hk, k0 + r, k0 + r < sp.n, d);
+      Ks[d * kTile + r] = x.x;
+      Ks[(d + 1) * kTile + r] = x.y;
+      Ks[(d + 2) * kTile + r] = x.z;
+      Ks[(d + 3) * kTile + r] = x.w;
+      const int rv = i / (DP / 4), dv = i % (DP / 4) * 4;  // V: neighbouring channels
+      *reinterpret_cast<float4*>(&Vs[rv * DP + dv]) = load4(p.v, p.vs, hk, k0 + rv, k0 + rv < sp.n, dv);
+    }
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 8
+    for (int d = 0; d < DP; ++d) {
+      const float4 q = *reinterpret_cast<const float4*>(&Qs[d * kTile + ty * 4]);
+      const float4 k = *reinterpret_cast<const float4*>(&Ks[d * kTile + tx * 4]);
+      const float qv[4] = {q.x, q.y, q.z, q.w}, kv[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = fmaf(qv[i], kv[j], s[i][j]);
+    }
+    if (!(k0 + kTile - 1 <= ra.hi && (k0 >= rz.lo || k0 + kTile - 1 < ra.sk))) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const RowKeys rk = row_keys(p, sp, sp.start + min(q0 + ty * 4 + i, q1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!rk.sees(k0 + tx * 4 + j)) s[i][j] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      mx = fmaxf(mx, m[i]);
+      const float mu = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[i] - mu);
+      m[i] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2f(s[i][j] - mu);
+        sum += s[i][j];
+      }
+      l[i] = fmaf(l[i], corr, sum);  // of this thread's keys; joined at the end
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) o[i][j] *= corr;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<float4*>(&Ps[(tx * 4 + j) * kTile + ty * 4]) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    __syncthreads();
+#pragma unroll 4
+    for (int k = 0; k < kTile; ++k) {
+      const float4 pv = *reinterpret_cast<const float4*>(&Ps[k * kTile + ty * 4]);
+      const float pr[4] = {pv.x, pv.y, pv.z, pv.w};
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const float4 v = *reinterpret_cast<const float4*>(&Vs[k * DP + c * 64 + tx * 4]);
+        const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][c * 4 + j] = fmaf(pr[i], vv[j], o[i][c * 4 + j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+    const int qi = q0 + ty * 4 + i;
+    if (qi >= p.Sq) continue;
+    const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+    T* dst = static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + qi * p.os[2];
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = c * 64 + tx * 4 + j;
+        if (d < p.D) dst[d * p.os[3]] = from_f32<T>(o[i][c * 4 + j] * inv);
+      }
+  }
+}
+
 // One CTA joins the shares of one row: groups of threads take shares in turn, a thread holds 4 channels (or
 // single ones where D is no multiple of 4), so that all the reads of a row are in flight at once.
 constexpr int kJoinThreads = 256;
@@ -274,18 +421,40 @@ static bool aligned16(const void* base, const int64_t* s, int64_t D) {
   return s[3] == 1 && D % 8 == 0 && (uintptr_t)base % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
 }
 
-// The tensor-core kernel computes tiles of 128 queries of a head whatever their number; the split kernel reads the
-// keys anew for each 16 rows of a key head.
-static bool takes_sm100(const mt_window_attention_desc& d) { return d.Sq > 32 && window_sm100_takes(d); }
-
 static bool takes_split(const mt_window_attention_desc& d) {
   return d.dtype != MT_F32 && aligned16(d.k, d.k_strides, d.D) && aligned16(d.v, d.v_strides, d.D);
+}
+
+// The tensor-core kernel (tiles of 256 queries of a head) or the split kernel (which reads the keys anew for each 16 rows
+// of a key head, but spreads them over the GPU)?  By the time that each takes: about 2 us per 128 keys and round of CTAs
+// (a prompt of 8192 in 4 rounds of 18 tiles: 148 us) behind a start of 5 us, against 4 TB/s of keys and values
+// (one token of 8 sequences: 131 MB in 32 us) behind 8 us.  33 queries of 2 heads over 4000 keys: 59 us and 12 us;
+// 64 of 8 heads over 900: 23 and 15; a padded batch of 3 x 1031 at 12 heads: 17 and 60.
+static bool takes_sm100(const mt_window_attention_desc& d) {
+  if (!window_sm100_takes(d)) return false;
+  if (!takes_split(d)) return true;
+  if (d.Sq <= 16) return false;  // a step of a few tokens: the start is what counts, and three tensor maps take the host longer
+  const double rounds = std::ceil((double)(d.B * d.H * ((d.Sq + 255) / 256)) / num_sms());
+  const double span = (double)span_keys(d.Sk, std::min<int64_t>(d.Sq, 256), d.causal, d.window, d.sinks);
+  const int64_t rows = d.Sq * (d.H / d.Hkv);
+  const double few = (double)span_keys(d.Sk, std::min(d.Sq, (16 + d.H / d.Hkv - 1) / (d.H / d.Hkv)), d.causal, d.window, d.sinks);
+  const double tiles_us = 5.0 + rounds * std::ceil(span / 128) * 2.0;
+  const double split_us = 8.0 + (double)(d.B * d.Hkv * ((rows + 15) / 16)) * few * d.D * 4.0 / 4e6;
+  return tiles_us < split_us;
+}
+
+// fp32 (and what neither of the two takes): tiles of 64 queries where they make a third of the SMs busy, else rows with
+// the keys split (12 queries of 4 heads over 600 keys: 79 us in 20 tiles; 3 x 1500 queries of 16 heads 0.9 ms in
+// tiles, 3.8 ms in rows).
+static bool takes_tiles(const mt_window_attention_desc& d) {
+  return d.Sq > 16 && d.B * d.H * ((d.Sq + kTile - 1) / kTile) * 3 >= num_sms();
 }
 
 static int window_splits(const mt_window_attention_desc& d) {
   if (takes_sm100(d)) return 1;
   if (takes_split(d))
     return split_count(d.B * d.Hkv, d.Sq * (d.H / d.Hkv), span_keys(d.Sk, d.Sq, d.causal, d.window, d.sinks));
+  if (takes_tiles(d)) return 1;
   return rows_splits(d.B, d.H, d.Hkv, d.Sq, d.Sk, d.causal, d.window, d.sinks);
 }
 
@@ -337,6 +506,25 @@ static int rows_launch(const AttnParams& p, cudaStream_t st) {
   return join_launch<T>(p, st);
 }
 
+template <typename T, int DP>
+static int tile_launch(const AttnParams& p, bool aligned, cudaStream_t st) {
+  constexpr int smem = (3 * DP + kTile) * kTile * 4;
+  auto kern = attn_tile_kernel<T, DP>;
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention tile smem attribute");
+    if (rc) return rc;
+    attr[dev & 63] = true;
+  }
+  const int64_t tiles = (p.Sq + kTile - 1) / kTile;
+  if ((int64_t)p.B * p.H > INT32_MAX || tiles > 65535)
+    return fail(MT_ERR_UNSUPPORTED, "window_attention: batch * heads or queries past the grid");
+  kern<<<dim3((unsigned)(p.B * p.H), (unsigned)tiles), 256, smem, st>>>(p, aligned);
+  return check_launch("attention_tile");
+}
+
 static int check_common(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window,
                         int64_t sinks, double scale, const char* what) {
   if (B < 0 || H <= 0 || Hkv <= 0 || Sq < 0 || Sk < 0 || D <= 0 || window < 0 || sinks < 0)
@@ -362,6 +550,12 @@ static int validate_window(const mt_window_attention_desc& d) {
   return MT_OK;
 }
 
+int window_attention_path(const mt_window_attention_desc& d) {
+  if (validate_window(d)) return 0;
+  return takes_sm100(d) ? MT_WINDOW_PATH_TC : takes_split(d) ? MT_WINDOW_PATH_SPLIT
+                      : takes_tiles(d) ? MT_WINDOW_PATH_TILES : MT_WINDOW_PATH_ROWS;
+}
+
 size_t window_attention_workspace(const mt_window_attention_desc& d) {
   if (validate_window(d) || d.B == 0 || d.Sq == 0) return 0;
   return part_bytes(window_splits(d), d.B * d.H * d.Sq, d.D);
@@ -375,8 +569,17 @@ static bool aligned4(const void* base, const int64_t* s, int64_t D, int es) {
 
 template <typename T>
 static int window_dispatch(const mt_window_attention_desc& d, const AttnParams& p, cudaStream_t st) {
-  if (aligned4(d.k, d.k_strides, d.D, sizeof(T)) && aligned4(d.v, d.v_strides, d.D, sizeof(T)))
-    return rows_launch<T, KV_ALIGNED>(p, st);
+  const bool kv4 = aligned4(d.k, d.k_strides, d.D, sizeof(T)) && aligned4(d.v, d.v_strides, d.D, sizeof(T));
+  if (takes_tiles(d)) {
+    const bool all4 = kv4 && aligned4(d.q, d.q_strides, d.D, sizeof(T));
+    switch ((d.D + 63) / 64) {
+      case 1: return tile_launch<T, 64>(p, all4, st);
+      case 2: return tile_launch<T, 128>(p, all4, st);
+      case 3: return tile_launch<T, 192>(p, all4, st);
+      default: return tile_launch<T, 256>(p, all4, st);
+    }
+  }
+  if (kv4) return rows_launch<T, KV_ALIGNED>(p, st);
   return rows_launch<T, KV_STRIDED>(p, st);
 }
 

@@ -17,6 +17,7 @@ import numpy as np
 import pytest
 
 import mtorch_b200 as mt
+from mtorch_b200 import _lib as L
 
 pytestmark = pytest.mark.gpu
 
@@ -200,6 +201,87 @@ WINDOW = [
     (1, 1, 1, 140, 140, 256, 33, 0, True),
     (1, 2, 1, 500, 900, 128, 1, 0, True),
 ]
+
+
+PATHS = {1: "tc", 2: "split", 3: "tiles", 4: "rows"}
+
+
+def path_of(q, k, v, window, sinks, causal=True, scale=0.125):
+    B, H, Sq, D = q.shape
+    return PATHS[L.lib().mt_cuda_window_attention_path(L.pack_window_attention(
+        B, H, k.shape[1], Sq, k.shape[2], D, q.dtype.code, causal, window or 0, sinks, 0, 0, q.data_ptr(), *q.stride(),
+        k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), q.data_ptr(), *q.stride(), scale))]
+
+
+# many heads and queries: the tensor-core tiles for 16-bit types, the fp32 tiles
+LARGE = [
+    # B, H, Hkv, Sq, Sk, D, window, sinks, causal
+    (1, 32, 32, 257, 257, 64, 100, 5, True),
+    (2, 24, 12, 300, 300, 128, 33, 0, True),
+    (1, 64, 8, 513, 640, 128, 300, 140, True),
+    (1, 48, 16, 400, 400, 40, None, 0, True),
+    (2, 32, 32, 129, 500, 80, 64, 3, False),
+    (1, 64, 64, 384, 384, 64, 1, 0, True),
+    (1, 64, 64, 700, 300, 64, 90, 2, True),  # queries before the first key see nothing
+    (3, 30, 10, 260, 131, 96, None, 7, False),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("case", LARGE)
+def test_window_attention_of_many_queries(case, dtype):
+    B, H, Hkv, Sq, Sk, D, window, sinks, causal = case
+    rng = np.random.default_rng(Sq * 3 + Sk)
+    q, qv = heads(rng, B, H, Sq, D, dtype)
+    k, kv = heads(rng, B, Hkv, Sk, D, dtype)
+    v, vv = heads(rng, B, Hkv, Sk, D, dtype, merged=False, extra=8)
+    assert path_of(q, k, v, window, sinks, causal) == ("tiles" if dtype == "float32" else "tc")
+    got = mt.window_attention(q, k, v, window, sinks, causal=causal)
+    want = attention_ref(qv, kv, vv, [Sk - Sq] * B, [Sk] * B, window, sinks, causal)
+    attention_close(got, want, dtype, np.abs(vv).max())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_of_many_queries_ragged(D, dtype):
+    """A padded batch: what stands past the lengths is NaN and infinity; scores that grow with the key (the running
+    maximum is raised in every tile) and an out= view that takes no vector stores."""
+    rng = np.random.default_rng(D)
+    B, H, Hkv, S, window, sinks = 6, 16, 8, 330, 150, 9
+    lengths = np.array([S, 0, 1, 129, 128, 200])
+    starts = np.zeros(B, np.int64)
+    q, qv = heads(rng, B, H, S, D, dtype)
+    kn, vn = rng.standard_normal((B, Hkv, S, D)), rng.standard_normal((B, Hkv, S, D))
+    kn += np.arange(S)[:, None] * 0.05
+    for b in range(B):
+        kn[b, :, lengths[b]:] = np.nan
+        vn[b, :, lengths[b]:] = [np.nan, np.inf, -np.inf, np.nan, 3, np.inf][b]
+    k, kv = rounded(kn, dtype)
+    v, vv = rounded(vn, dtype)
+    assert path_of(q, k, v, window, sinks) == ("tiles" if dtype == "float32" else "tc")
+    store = mt.zeros(B, S, H * D + 3, dtype=dtype, device="cuda")
+    out = store._view((B, H, S, D), (S * (H * D + 3), D, H * D + 3, 1))
+    mt.window_attention(q, k, v, window, sinks, starts=i32(starts), lengths=i32(lengths), out=out)
+    want = attention_ref(qv, kv, vv, starts, lengths, window, sinks, True)
+    # keys of up to 16: the fp32 scores of D products of up to 60 move the result by up to 1e-3
+    np.testing.assert_allclose(host(out), want, rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-3) * 5.0)
+    assert (host(store)[..., H * D:] == 0).all()
+
+
+def test_window_attention_paths():
+    """Few queries take the split keys, unaligned rows and a negative scale the others."""
+    rng = np.random.default_rng(0)
+    q, _ = heads(rng, 1, 4, 1, 64, "bfloat16")
+    k, _ = heads(rng, 1, 2, 100, 64, "bfloat16")
+    assert path_of(q, k, k, 10, 0) == "split"
+    odd, _ = heads(rng, 1, 2, 100, 64, "bfloat16", extra=1)
+    assert path_of(q, odd, odd, 10, 0) == "rows"
+    q, _ = heads(rng, 2, 64, 300, 64, "bfloat16")
+    k, _ = heads(rng, 2, 64, 300, 64, "bfloat16")
+    assert path_of(q, k, k, 100, 0) == "tc"
+    assert path_of(q, k, k, 100, 0, scale=-1.0) == "split"
+    odd, _ = heads(rng, 2, 64, 300, 64, "bfloat16", extra=1)
+    assert path_of(q, odd, odd, 100, 0) == "tiles"
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
