@@ -150,6 +150,8 @@ def packer(desc):
 
 
 pack_rotary = packer(RotaryDesc)
+pack_kv_cache4 = packer(KvCache4Desc)
+pack_strides = struct.Struct("@4q").pack
 pack_window_attention = packer(WindowAttentionDesc)
 pack_kv_cache4_attention = packer(KvCache4AttentionDesc)
 pack_linear_weight4 = packer(LinearWeight4Desc)
@@ -236,10 +238,8 @@ SIGNATURES = {
     "mt_cuda_window_attention_workspace_size": (C.c_size_t, [VP]),
     "mt_cuda_window_attention": (C.c_int, [VP, VP, C.c_size_t, VP]),
     "mt_cuda_window_attention_path": (C.c_int, [VP]),
-    "mt_cuda_kv_cache4_append": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
-                                           I64, VP, VP]),
-    "mt_cuda_kv_cache4_read": (C.c_int, [C.POINTER(KvCache4Desc), VP, _P64, VP, _P64, C.c_int, I64, I64, VP, I64,
-                                         I64, VP, VP]),
+    "mt_cuda_kv_cache4_append": (C.c_int, [VP, VP, VP, VP, VP, C.c_int, I64, I64, VP, I64, I64, VP, VP]),
+    "mt_cuda_kv_cache4_read": (C.c_int, [VP, VP, VP, VP, VP, C.c_int, I64, I64, VP, I64, I64, VP, VP]),
     "mt_cuda_kv_cache4_attention_workspace_size": (C.c_size_t, [VP]),
     "mt_cuda_kv_cache4_attention": (C.c_int, [VP, VP, C.c_size_t, VP]),
     "mt_cuda_linear_weight4_workspace_size": (C.c_size_t, [VP]),

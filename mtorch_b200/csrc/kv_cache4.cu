@@ -20,12 +20,12 @@ struct FastDiv {
 };
 
 struct Cache4Params {
-  FastDiv by_words, by_inner;  // D / 8; heads (append), tokens (read)
+  FastDiv by_words, by_inner;  // D / 8; heads (append), threads' tokens (read)
   const int32_t* table;
   int64_t table_stride;
   int max_pages, page_shift, num_pages;
   int Hkv, D, T;
-  int items;  // T * Hkv * D / 8: words of one sequence
+  int items;  // ceil(T / tokens of a thread) * Hkv * D / 8: threads of one sequence
   const int32_t* starts;
   int32_t* words[2];
   __half2* scales[2];  // (scale, zero)
@@ -63,7 +63,60 @@ __device__ __forceinline__ Vec8<T> load8(const T* src, int64_t st, bool vec) {
   return x;
 }
 
-// A thread takes the same word of K and of V: one look into the table, two values' loads in flight.
+constexpr int kAppendTokens = 1, kReadTokens = 4;  // consecutive tokens of a thread
+
+// The code word and (scale, zero) of eight channels of a group of 64, whose other channels neighbouring lanes hold.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const Vec8<T>& in, __half2& scale_zero) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(in.v[j]);
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) {
+    lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, x[j]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+  const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
+  scale_zero = __halves2half2(scale, zero);
+  const float z = __half2float(zero), s = __half2float(scale);
+  // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22 of
+  // itself of the divided one, so it rounds to the same code unless it is that near to a tie (within 2^-18 up to
+  // 15.5); then the word's quotients are divided as the definition says.  1.5 * 2^23 added to a number rounds it to a
+  // whole one, which stands in the sum's low bits.
+  constexpr float kRound = 12582912.f;
+  uint32_t word = 0;
+  if (s > 0.f) {
+    const float inv = 1.f / s;
+    float tie = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inv), 0.f), 15.f);
+      const float r = __fadd_rn(q, kRound);
+      tie = fmaxf(tie, fabsf(q - (r - kRound)));
+      word |= (__float_as_uint(r) & 15u) << (4 * j);
+    }
+    if (tie > 0.5f - 3.8e-6f) {
+      word = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
+        word |= (uint32_t)c << (4 * j);
+      }
+    }
+  }
+  return word;
+}
+
+// A thread takes the same word of K and of V: the index arithmetic and the look into the table are shared.  18 MB of keys and
+// values take 14, 16, 18 us with 1, 2, 4 tokens a thread: the arithmetic of a word (about 100 instructions)
+// wants warps more than loads in flight.  Reading back, 8 us with 4 tokens, 10.5 with one.
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -72,60 +125,29 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Params p
   const bool live = idx < (uint32_t)p.items;  // whole groups of 8 threads are live or not
   const uint32_t i = live ? idx : 0;
   const uint32_t r = p.by_words.div(i), w = i - r * W;
-  const int t = p.by_inner.div(r), h = r - (uint32_t)t * p.Hkv;
-  Vec8<T> in[2];
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv)
-    in[kv] = load8<T>(static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
-                          (int64_t)w * 8 * p.st[kv][3], p.st[kv][3], p.vec);
-  const int64_t row = live ? cache4_row(p, b, h, t) : -1;
+  const int tq = p.by_inner.div(r), h = r - (uint32_t)tq * p.Hkv, t0 = tq * kAppendTokens;
+  Vec8<T> in[2][kAppendTokens];
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    float x[8];
+    const T* src = static_cast<const T*>(p.in[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t0 * p.st[kv][2] +
+                   (int64_t)w * 8 * p.st[kv][3];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(in[kv].v[j]);
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) {
-      lo = fminf(lo, x[j]);
-      hi = fmaxf(hi, x[j]);
+    for (int u = 0; u < kAppendTokens; ++u) {
+      in[kv][u] = load8<T>(src, p.st[kv][3], p.vec);
+      if (t0 + u + 1 < p.T) src += p.st[kv][2];  // (tokens past the last repeat it)
     }
+  }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-    const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
-    const float z = __half2float(zero), s = __half2float(scale);
-    // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22
-    // of itself of the divided one, so it rounds to the same code unless it is that near to a tie (within 2^-18 up to
-    // 15.5); then the word's quotients are divided as the definition says.  1.5 * 2^23 added to a number rounds it to
-    // a whole one, which stands in the sum's low bits.
-    constexpr float kRound = 12582912.f;
-    uint32_t word = 0;
-    if (s > 0.f) {
-      const float inv = 1.f / s;
-      float tie = 0.f;
+  for (int u = 0; u < kAppendTokens; ++u) {
+    const int64_t row = live && t0 + u < p.T ? cache4_row(p, b, h, t0 + u) : -1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inv), 0.f), 15.f);
-        const float r2 = __fadd_rn(q, kRound);
-        tie = fmaxf(tie, fabsf(q - (r2 - kRound)));
-        word |= (__float_as_uint(r2) & 15u) << (4 * j);
+    for (int kv = 0; kv < 2; ++kv) {
+      __half2 sz;
+      const uint32_t word = quantise8<T>(in[kv][u], sz);
+      if (row >= 0) {
+        p.words[kv][row * W + w] = (int32_t)word;
+        if ((w & 7) == 0) p.scales[kv][row * (W / 8) + (w >> 3)] = sz;
       }
-      if (tie > 0.5f - 3.8e-6f) {
-        word = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
-          word |= (uint32_t)c << (4 * j);
-        }
-      }
-    }
-    if (row >= 0) {
-      p.words[kv][row * W + w] = (int32_t)word;
-      if ((w & 7) == 0) p.scales[kv][row * (W / 8) + (w >> 3)] = __halves2half2(scale, zero);
     }
   }
 }
@@ -137,31 +159,39 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) 
   if (idx >= (uint32_t)p.items) return;
   const uint32_t W = p.D / 8;
   const uint32_t r = p.by_words.div(idx), w = idx - r * W;
-  const int h = p.by_inner.div(r), t = r - (uint32_t)h * p.T;
-  const int64_t row = cache4_row(p, b, h, t);
-  uint32_t word[2] = {0, 0};
-  float2 sz[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  if (row >= 0) {
+  const int h = p.by_inner.div(r), t0 = (r - (uint32_t)h * p.by_inner.d) * kReadTokens;
+  uint32_t word[2][kReadTokens];
+  __half2 sz[2][kReadTokens];
+#pragma unroll
+  for (int u = 0; u < kReadTokens; ++u) {
+    const int64_t row = t0 + u < p.T ? cache4_row(p, b, h, t0 + u) : -1;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      word[kv] = (uint32_t)p.words[kv][row * W + w];
-      sz[kv] = __half22float2(p.scales[kv][row * (W / 8) + (w >> 3)]);
+      word[kv][u] = row >= 0 ? (uint32_t)p.words[kv][row * W + w] : 0u;
+      sz[kv][u] = row >= 0 ? p.scales[kv][row * (W / 8) + (w >> 3)] : __half2(__ushort_as_half(0), __ushort_as_half(0));
     }
   }
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    T* dst = static_cast<T*>(p.out[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t * p.st[kv][2] +
+    T* dst = static_cast<T*>(p.out[kv]) + b * p.st[kv][0] + h * p.st[kv][1] + t0 * p.st[kv][2] +
              (int64_t)w * 8 * p.st[kv][3];
-    Vec8<T> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)  // 2^23 | code as a number, minus 2^23: the code
-      o.v[j] = from_f32<T>(fmaf(__uint_as_float(0x4b000000u | ((word[kv] >> (4 * j)) & 15u)) - 8388608.f, sz[kv].x, sz[kv].y));
-    if (p.vec) {
+    for (int u = 0; u < kReadTokens; ++u) {
+      if (t0 + u >= p.T) break;
+      const float2 f = __half22float2(sz[kv][u]);
+      Vec8<T> o;
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(o.v)[j];
-    } else {
+      for (int j = 0; j < 8; ++j)  // 2^23 | code as a number, minus 2^23: the code
+        o.v[j] = from_f32<T>(fmaf(__uint_as_float(0x4b000000u | ((word[kv][u] >> (4 * j)) & 15u)) - 8388608.f, f.x, f.y));
+      if (p.vec) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dst[j * p.st[kv][3]] = o.v[j];
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+          reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(o.v)[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dst[j * p.st[kv][3]] = o.v[j];
+      }
+      dst += p.st[kv][2];
     }
   }
 }
@@ -184,7 +214,7 @@ int validate_kv_cache4(const mt_kv_cache4& c) {
 
 static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v,
                          const int64_t* vs, int dtype, int64_t B, int64_t T, const int32_t* table,
-                         int64_t table_stride, int64_t max_pages, const int32_t* starts, const char* what) {
+                         int64_t table_stride, int64_t max_pages, const int32_t* starts, int tokens, const char* what) {
   int rc = validate_kv_cache4(c);
   if (rc) return rc;
   if (dtype != MT_F32 && dtype != MT_BF16 && dtype != MT_F16) return fail(MT_ERR_UNSUPPORTED, "%s: dtype", what);
@@ -196,7 +226,7 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   p.num_pages = (int)c.num_pages;
   p.Hkv = (int)c.Hkv; p.D = (int)c.D; p.T = (int)T;
   if (B > 65535 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
-  p.items = (int)(T * c.Hkv * (c.D / 8));
+  p.items = (int)((T + tokens - 1) / tokens * c.Hkv * (c.D / 8));
   p.starts = starts;
   p.by_words = FastDiv((uint32_t)(c.D / 8));
   p.words[0] = c.k_words; p.words[1] = c.v_words;
@@ -216,7 +246,8 @@ int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks
                          int dtype, int64_t B, int64_t T, const int32_t* table, int64_t table_stride,
                          int64_t max_pages, const int32_t* starts, cudaStream_t st) {
   Cache4Params p{};
-  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_append");
+  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, kAppendTokens,
+                         "kv_cache4_append");
   if (rc || B == 0 || p.items == 0) return rc;
   p.in[0] = k; p.in[1] = v;
   p.by_inner = FastDiv((uint32_t)c.Hkv);
@@ -233,10 +264,11 @@ int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* 
                        int64_t B, int64_t T, const int32_t* table, int64_t table_stride, int64_t max_pages,
                        const int32_t* starts, cudaStream_t st) {
   Cache4Params p{};
-  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, "kv_cache4_read");
+  int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, kReadTokens,
+                         "kv_cache4_read");
   if (rc || B == 0 || p.items == 0) return rc;
   p.out[0] = k; p.out[1] = v;
-  p.by_inner = FastDiv((uint32_t)T);
+  p.by_inner = FastDiv((uint32_t)((T + kReadTokens - 1) / kReadTokens));
   dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)B);
   switch (dtype) {
     case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;

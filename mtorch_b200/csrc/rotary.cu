@@ -171,7 +171,7 @@ static int rotary_launch(const mt_rotary_desc& d, RotaryParams& p, cudaStream_t 
   const int64_t blocks = (items + 255) / 256;
   if (blocks > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "rotary: too many elements");
   // heads are shared out over CTAs until the GPU is full: few tokens leave nothing else to share
-  int64_t parts = std::min<int64_t>(heads, std::max<int64_t>(1, (8LL * num_sms() + blocks - 1) / blocks));
+  int64_t parts = std::min<int64_t>(heads, std::max<int64_t>(1, (12LL * num_sms() + blocks - 1) / blocks));
   p.heads_per_block = (int)((heads + parts - 1) / parts);
   dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block));
   const bool inter = d.interleaved != 0;

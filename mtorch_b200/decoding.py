@@ -8,7 +8,6 @@ takes them; `out=` takes any view of the right shape and writes the result there
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 
 import numpy as np
@@ -46,13 +45,12 @@ def _run(fn, size_fn, desc, t, what):
         L.check(rc, what)
 
 
-def _require_int32(what, shape, **named):
-    """Index tensors: int32 on the device, contiguous, of the given shape."""
-    for name, t in named.items():
-        if t.dtype is not int32 or t.device.type != "cuda":
-            raise ValueError(f"{what}: {name} has to be an int32 tensor on the cuda device")
-        if t._shape != shape or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} has to be contiguous of shape {list(shape)}, got {list(t._shape)}")
+def _require_int32(what, B, name, t):
+    """Index tensors of a batch: int32 on the device, contiguous, one value a sequence."""
+    if t.dtype is not int32 or t.device.type != "cuda":
+        raise ValueError(f"{what}: {name} has to be an int32 tensor on the cuda device")
+    if t._shape != (B,) or (t._strides != (1,) and B > 1):
+        raise ValueError(f"{what}: {name} has to be contiguous of shape [{B}], got {list(t._shape)}")
 
 
 def _check_out(out, shape, like, what):
@@ -181,9 +179,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int | None, sinks:
         raise ValueError(f"{what}: number of heads in key/value must divide number of heads in query")
     w = _window_arg(window, sinks, what)
     if starts is not None:
-        _require_int32(what, (B,), starts=starts)
+        _require_int32(what, B, "starts", starts)
     if lengths is not None:
-        _require_int32(what, (B,), lengths=lengths)
+        _require_int32(what, B, "lengths", lengths)
     if out is None:
         out = _new_heads(B, H, Sq, D, q)
     else:
@@ -231,7 +229,7 @@ class KVCache4:
         self.device = k_words.device
         self._fields = (pages, page, heads, w * 8, k_words.data_ptr(), k_scales.data_ptr(), v_words.data_ptr(),
                         v_scales.data_ptr())
-        self._desc = C.byref(L.KvCache4Desc(*self._fields))
+        self._desc = L.pack_kv_cache4(*self._fields)
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, heads: int, dim: int, device="cuda") -> "KVCache4":
@@ -265,9 +263,9 @@ def _cache_move(cache, k, v, table, starts, T, fn, what):
         raise ValueError(f"{what}: k and v have to be [batch, {cache.heads}, {T}, {cache.dim}], got {list(k._shape)} "
                          f"and {list(v._shape)}")
     _check_table(cache, table, B, what)
-    _require_int32(what, (B,), starts=starts)
-    _check(fn(cache._desc, _ptr(k), L.I64_4(*k._strides), _ptr(v), L.I64_4(*v._strides), k.dtype.code, B, T, _ptr(table),
-              table._strides[0], table._shape[1], _ptr(starts), stream_ptr(cache.device.index or 0)), what)
+    _require_int32(what, B, "starts", starts)
+    _check(fn(cache._desc, _ptr(k), L.pack_strides(*k._strides), _ptr(v), L.pack_strides(*v._strides), k.dtype.code, B, T,
+              _ptr(table), table._strides[0], table._shape[1], _ptr(starts), stream_ptr(cache.device.index or 0)), what)
 
 
 def kv_cache_append(cache: KVCache4, k: Tensor, v: Tensor, block_table: Tensor, starts: Tensor) -> None:
@@ -321,7 +319,7 @@ def kv_cache_attention(q: Tensor, cache: KVCache4, block_table: Tensor, lengths:
         raise NotImplementedError(f"{what}: dtype {q.dtype.name} is not supported (bfloat16 or float16)")
     w = _window_arg(window, sinks, what)
     _check_table(cache, block_table, B, what)
-    _require_int32(what, (B,), lengths=lengths)
+    _require_int32(what, B, "lengths", lengths)
     if out is None:
         out = _new_heads(B, H, Sq, D, q)
     else:
