@@ -4,7 +4,9 @@ The public names mirror mtorch's torch-shaped API (mtorch/__init__.py) for the d
 ``Tensor.to('cuda')``, ``nn.Linear/Conv2d/GroupNorm/LayerNorm``, ``nn.functional.*``
 (``scaled_dot_product_attention``, ``conv2d``, ``linear``, ``group_norm``, ``layer_norm``,
 ``softmax``, ``silu``, ``gelu``), ``matmul/bmm/addmm/baddbmm``, ``manual_seed/randn/rand`` (bit-
-compatible with mtorch's generator) and ``cuda.*``.  All device compute runs in
+compatible with mtorch's generator) and ``cuda.*``.  Beyond the reference it has the operators of a
+causal decoder (``rotary_embedding``, ``window_attention``, ``KVCache4`` with ``kv_cache_*``, ``Weight4`` with
+``linear_weight4``; ``decoding.py``) and ``from_device_memory`` for other libraries' memory.  All device compute runs in
 ``libmtorch_cuda.so`` (hand-written sm_100a kernels behind the C ABI of include/mtorch_cuda.h).
 """
 from __future__ import annotations
