@@ -428,8 +428,8 @@ static bool takes_split(const mt_window_attention_desc& d) {
 // The tensor-core kernel (tiles of 256 queries of a head) or the split kernel (which reads the keys anew for each 16 rows
 // of a key head, but spreads them over the GPU)?  By the time that each takes: about 2 us per 128 keys and round of CTAs
 // (a prompt of 8192 in 4 rounds of 18 tiles: 148 us) behind a start of 5 us, against 4 TB/s of keys and values
-// (one token of 8 sequences: 131 MB in 32 us) behind 8 us.  33 queries of 2 heads over 4000 keys: 59 us and 12 us;
-// 64 of 8 heads over 900: 23 and 15; a padded batch of 3 x 1031 at 12 heads: 17 and 60.
+// (one token of 8 sequences: 131 MB in 32 us) behind 8 us.  Tiles and split keys: 33 queries of 2 heads over 4000 keys 60
+// and 15 us; 100 of 8 heads over 1000 25 and 17; 300 of 16 heads over 300 10 and 29; 2048 of 16 heads 37 and 242.
 static bool takes_sm100(const mt_window_attention_desc& d) {
   if (!window_sm100_takes(d)) return false;
   if (!takes_split(d)) return true;
@@ -444,8 +444,8 @@ static bool takes_sm100(const mt_window_attention_desc& d) {
 }
 
 // fp32 (and what neither of the two takes): tiles of 64 queries where they make a third of the SMs busy, else rows with
-// the keys split (12 queries of 4 heads over 600 keys: 79 us in 20 tiles; 3 x 1500 queries of 16 heads 0.9 ms in
-// tiles, 3.8 ms in rows).
+// the keys split.  Tiles and rows: 300 queries of 4 heads over 600 keys 78 and 41 us (20 tiles), of 16 heads 78 and 95
+// (80 tiles); 3 x 1500 of 16 heads 0.9 and 2.8 ms.
 static bool takes_tiles(const mt_window_attention_desc& d) {
   return d.Sq > 16 && d.B * d.H * ((d.Sq + kTile - 1) / kTile) * 3 >= num_sms();
 }

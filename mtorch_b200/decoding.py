@@ -164,7 +164,8 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int | None, sinks:
     Query i of sequence b is at position p = starts[b] + i (default Sk - Sq + i).  It sees key j below
     lengths[b] (default Sk) when j <= p and (p - j < window or j < sinks); without `causal` when
     |p - j| < window or j < sinks.  `window=None`: no window.  A query that sees no key gets zeros.
-    Keys at lengths[b] and beyond may hold anything.  H may be a multiple of Hkv (shared key
+    Keys at lengths[b] and beyond may hold anything; below it the values have to be finite (an infinity or
+    NaN can reach neighbouring queries that do not see its key).  H may be a multiple of Hkv (shared key
     heads).  `starts`, `lengths`: int32 [B] on the device."""
     what = "window_attention"
     _require_cuda(q, k, v)

@@ -518,3 +518,92 @@ def test_linear_weight4_views():
     z = mt.linear_weight4(wide[:, :K].reshape(2, 3, K), p)
     np.testing.assert_array_equal(host(z).reshape(6, N), got[:, 3:43])
     assert mt.linear_weight4(wide[:0, :K], p).shape == (0, N)
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes of zero, tables and offsets past 32 bits
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_sizes_of_zero(dtype):
+    rng = np.random.default_rng(0)
+    q, _ = heads(rng, 2, 4, 3, 64, dtype)
+    none = mt.zeros(2, 2, 0, 64, dtype=dtype, device="cuda")
+    for Sq in (3, 0):
+        o = mt.window_attention(q[:, :, :Sq], none, none, 5, 2)
+        assert o.shape == (2, 4, Sq, 64) and (host(o) == 0).all()
+    many, _ = heads(rng, 1, 64, 300, 64, dtype)
+    o = mt.window_attention(many, none[:1], none[:1], 5, 2)
+    assert (host(o) == 0).all()
+    freq = mt.rotary_frequencies((4,))
+    r = mt.rotary_embedding(q[:, :, :0], None, mt.zeros(1, 0, dtype="int32", device="cuda"), freq, (4,))
+    assert r.shape == (2, 4, 0, 64)
+    cache = mt.KVCache4.empty(2, 16, 2, 64)
+    table, zero = i32([[0], [1]]), i32([0, 0])
+    mt.kv_cache_append(cache, none, none, table, zero)
+    k, v = mt.kv_cache_read(cache, table, zero, 0)
+    assert k.shape == (2, 2, 0, 64)
+    if dtype == "bfloat16":
+        assert (host(mt.kv_cache_attention(q, cache, table, zero)) == 0).all()
+        empty = mt.zeros(2, 0, dtype="int32", device="cuda")  # a table of no pages
+        assert (host(mt.kv_cache_attention(q, cache, empty, i32([5, 7]))) == 0).all()
+
+
+def test_table_with_a_row_pitch_and_shared_pages():
+    """Two sequences share their first pages (a forked prompt); the table is a view of a wider one."""
+    rng = np.random.default_rng(2)
+    H, D, page = 2, 128, 16
+    cache = mt.KVCache4.empty(8, page, H, D)
+    wide = np.full((2, 9), 77, np.int32)
+    wide[:, 1:5] = [[0, 1, 2, 3], [0, 1, 4, 5]]
+    table = i32(wide)[:, 1:5]
+    k, kv = rounded(rng.standard_normal((2, H, 64, D)), "bfloat16")
+    v, vv = rounded(rng.standard_normal((2, H, 64, D)), "bfloat16")
+    mt.kv_cache_append(cache, k[:1, :, :32], v[:1, :, :32], table[:1], i32([0]))       # the shared prompt
+    mt.kv_cache_append(cache, k[:, :, 32:], v[:, :, 32:], table, i32([32, 32]))         # what follows, apart
+    kq, vq = quantised(kv), quantised(vv)
+    kq[1, :, :32], vq[1, :, :32] = kq[0, :, :32], vq[0, :, :32]
+    q, qv = heads(rng, 2, 8, 1, D, "bfloat16")
+    got = mt.kv_cache_attention(q, cache, table, i32([64, 50]))
+    want = attention_ref(qv, kq, vq, [63, 49], [64, 50], None, 0, True)
+    np.testing.assert_allclose(host(got), want, rtol=2.0 ** -8, atol=(2.0 ** -8 + 1e-4) * 5)
+
+
+def test_cache_past_32_bits():
+    """A page whose words begin 4.3 GB into the arrays."""
+    rng = np.random.default_rng(4)
+    page, D, pages = 1024, 256, 33000  # 128 bytes a token: 4.3e9 bytes of words each for K and V
+    words = [mt.empty(pages, 1, page, D // 8, dtype="int32", device="cuda") for _ in range(2)]
+    scales = [mt.empty(pages, 1, page, D // 64, 2, dtype="float16", device="cuda") for _ in range(2)]
+    cache = mt.KVCache4(words[0], scales[0], words[1], scales[1])
+    table = i32([[pages - 1, pages - 2]])
+    k, kv = rounded(rng.standard_normal((1, 1, 1100, D)), "bfloat16")
+    v, vv = rounded(rng.standard_normal((1, 1, 1100, D)), "bfloat16")
+    mt.kv_cache_append(cache, k, v, table, i32([0]))
+    gk, gv = mt.kv_cache_read(cache, table, i32([1000]), 100, dtype="float32")
+    np.testing.assert_allclose(host(gk), quantised(kv)[:, :, 1000:], rtol=2.0 ** -23, atol=1e-6)
+    np.testing.assert_allclose(host(gv), quantised(vv)[:, :, 1000:], rtol=2.0 ** -23, atol=1e-6)
+    q, qv = heads(rng, 1, 2, 1, D, "bfloat16")
+    got = mt.kv_cache_attention(q, cache, table, i32([1100]))
+    want = attention_ref(qv, quantised(kv), quantised(vv), [1099], [1100], None, 0, True)
+    np.testing.assert_allclose(host(got), want, rtol=2.0 ** -8, atol=(2.0 ** -8 + 1e-4) * 5)
+
+
+@pytest.mark.parametrize("Sq,H", [(1, 4), (300, 64)])
+def test_strides_past_32_bits(Sq, H):
+    """Sequences that lie 2^31 elements apart in one buffer."""
+    rng = np.random.default_rng(Sq)
+    S, D, far = 320, 64, (1 << 31) + 64
+    buf = mt.empty(far + H * S * D, dtype="bfloat16", device="cuda")
+    q, qv = heads(rng, 2, H, Sq, D, "bfloat16")
+    k, kv = rounded(rng.standard_normal((2, H, S, D)), "bfloat16")
+    view = buf._view((2, H, S, D), (far, S * D, D, 1))
+    view.copy_(k)
+    got = mt.window_attention(q, view, view, 100, 3)
+    want = attention_ref(qv, kv, kv, [S - Sq] * 2, [S] * 2, 100, 3, True)
+    attention_close(got, want, "bfloat16", np.abs(kv).max())
+    freq = mt.rotary_frequencies((16, 16))
+    pos = rng.integers(0, 500, (2, S)).astype(np.int32)
+    mt.rotary_embedding(view, None, i32(pos), freq, (16, 16), out=view)
+    want = rotary_ref(kv, pos, freq.numpy(), (16, 16), False, False)
+    np.testing.assert_allclose(host(view[1:]), want[1:], rtol=2 * U["bfloat16"], atol=2.0 ** -20 * np.abs(kv).max())
