@@ -155,51 +155,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     return;
   }
 
-  // Q fragments: dense, 8 channels at 32 c + 8 t of row n; paged, the channel order of the codes' pairs
-  uint32_t qf[NT][2 * DC][4];
-  float qsum[NT][DC][2];
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    const int r = r0 + 8 * x + n;
-    const bool live = 8 * x + n < nr;
-    const T* src = static_cast<const T*>(p.q);
-    if (live) src += b * p.qs[0] + (int64_t)(hk * p.g + r % p.g) * p.qs[1] + (int64_t)(r / p.g) * p.qs[2];
-#pragma unroll
-    for (int c = 0; c < 2 * DC; ++c) {
-      const int base = PAGED ? (c >> 1) * 64 + t * 16 + (c & 1) * 8 : c * 32 + t * 8;
-      float v[8];
-      uint16_t u[8];
-      alignas(16) T raw[8];
-      if (p.q_vec) {  // (D is a multiple of 8)
-        *reinterpret_cast<uint4*>(raw) = live && base < p.D ? __ldg(reinterpret_cast<const uint4*>(src + base)) : make_uint4(0, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) raw[j] = live && base + j < p.D ? src[(base + j) * p.qs[3]] : from_f32<T>(0.f);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = to_f32<T>(raw[j]);
-        if (p.scale_log2 < 0.f) v[j] = -v[j];  // the maximum is taken of unscaled scores
-        const float f = !PAGED ? 1.f : (F16 ? 1.f : kPow64) * (j & 1 ? 0.0625f : 1.f);
-        const T h = from_f32<T>(v[j] * f);
-        u[j] = *reinterpret_cast<const uint16_t*>(&h);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        qf[x][c][j] = PAGED ? (u[j] | (uint32_t)u[j + 4] << 16) : (u[2 * j] | (uint32_t)u[2 * j + 1] << 16);
-      if (PAGED) {
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
-        s *= F16 ? 1.f / 16777216.f : 1.f / kPow69;  // the unit of q.c below
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-        qsum[x][c >> 1][0] = (c & 1) ? qsum[x][c >> 1][0] + s0 : s0;
-        qsum[x][c >> 1][1] = (c & 1) ? qsum[x][c >> 1][1] + s1 : s1;
-      }
-    }
-  }
   // keys that each row sees; keys that all rows see (ra.hi, rz.lo, ra.sk), that any row sees (ra.lo, rz.hi, rz.sk)
   if (threadIdx.x < ROWS) srk[threadIdx.x] = row_keys(p, sp, sp.start + (r0 + min((int)threadIdx.x, nr - 1)) / p.g);
   const RowKeys ra = row_keys(p, sp, pmin), rz = row_keys(p, sp, pmax);
@@ -338,6 +293,51 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     if (PAGED && i0 < i1) {
       missing_steps |= (uint32_t)(row_next == kNoRow) << s;
       row_next = cache_row(i + (s + 1) * kSplitWarps);
+    }
+  }
+  // Q fragments (while the first keys are on their way): dense, 8 channels at 32 c + 8 t of row n; paged, the channel order of the codes' pairs
+  uint32_t qf[NT][2 * DC][4];
+  float qsum[NT][DC][2];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    const int r = r0 + 8 * x + n;
+    const bool live = 8 * x + n < nr;
+    const T* src = static_cast<const T*>(p.q);
+    if (live) src += b * p.qs[0] + (int64_t)(hk * p.g + r % p.g) * p.qs[1] + (int64_t)(r / p.g) * p.qs[2];
+#pragma unroll
+    for (int c = 0; c < 2 * DC; ++c) {
+      const int base = PAGED ? (c >> 1) * 64 + t * 16 + (c & 1) * 8 : c * 32 + t * 8;
+      float v[8];
+      uint16_t u[8];
+      alignas(16) T raw[8];
+      if (p.q_vec) {  // (D is a multiple of 8)
+        *reinterpret_cast<uint4*>(raw) = live && base < p.D ? __ldg(reinterpret_cast<const uint4*>(src + base)) : make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) raw[j] = live && base + j < p.D ? src[(base + j) * p.qs[3]] : from_f32<T>(0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = to_f32<T>(raw[j]);
+        if (p.scale_log2 < 0.f) v[j] = -v[j];  // the maximum is taken of unscaled scores
+        const float f = !PAGED ? 1.f : (F16 ? 1.f : kPow64) * (j & 1 ? 0.0625f : 1.f);
+        const T h = from_f32<T>(v[j] * f);
+        u[j] = *reinterpret_cast<const uint16_t*>(&h);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        qf[x][c][j] = PAGED ? (u[j] | (uint32_t)u[j + 4] << 16) : (u[2 * j] | (uint32_t)u[2 * j + 1] << 16);
+      if (PAGED) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+        s *= F16 ? 1.f / 16777216.f : 1.f / kPow69;  // the unit of q.c below
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+        qsum[x][c >> 1][0] = (c & 1) ? qsum[x][c >> 1][0] + s0 : s0;
+        qsum[x][c >> 1][1] = (c & 1) ? qsum[x][c >> 1][1] + s1 : s1;
+      }
     }
   }
   int stage = 0;
