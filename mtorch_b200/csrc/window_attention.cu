@@ -558,7 +558,9 @@ int window_attention_path(const mt_window_attention_desc& d) {
 
 size_t window_attention_workspace(const mt_window_attention_desc& d) {
   if (validate_window(d) || d.B == 0 || d.Sq == 0) return 0;
-  return part_bytes(window_splits(d), d.B * d.H * d.Sq, d.D);
+  const int splits = window_splits(d);
+  if (takes_split(d) && split_joins_in_cluster(d.B * d.Hkv, d.Sq * (d.H / d.Hkv), splits)) return 0;
+  return part_bytes(splits, d.B * d.H * d.Sq, d.D);
 }
 
 // 4 channels are one aligned vector
@@ -599,14 +601,14 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
     p.qs[i] = d.q_strides[i]; p.ks[i] = d.k_strides[i]; p.vs[i] = d.v_strides[i]; p.os[i] = d.o_strides[i];
   }
   p.splits = window_splits(d);
-  if (ws_bytes < window_attention_workspace(d) || (p.splits > 1 && !ws))
-    return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
+  const size_t need = window_attention_workspace(d);
+  if (need && (!ws || ws_bytes < need)) return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
   bind_workspace(p, ws);
   if (takes_sm100(d)) return run_window_sm100(d, p, st);
   if (takes_split(d)) {
     p.q_vec = aligned16(d.q, d.q_strides, d.D);
     rc = run_split_attention(p, d.dtype, false, st);
-    return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
+    return rc || p.splits == 1 || p.cluster ? rc : join(p, d.dtype, st);
   }
   switch (d.dtype) {
     case MT_F32: return window_dispatch<float>(d, p, st);
@@ -631,7 +633,9 @@ static int validate_cache_attention(const mt_kv_cache4_attention_desc& d) {
 
 size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d) {
   if (validate_cache_attention(d) || d.B == 0 || d.Sq == 0) return 0;
-  return part_bytes(cache_splits(d), d.B * d.H * d.Sq, d.cache.D);
+  const int splits = cache_splits(d);
+  if (split_joins_in_cluster(d.B * d.cache.Hkv, d.Sq * (d.H / d.cache.Hkv), splits)) return 0;
+  return part_bytes(splits, d.B * d.H * d.Sq, d.cache.D);
 }
 
 int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -657,12 +661,12 @@ int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size
   p.num_pages = (int)d.cache.num_pages;
   p.page_shift = __builtin_ctzll((unsigned long long)d.cache.page_size);
   p.splits = cache_splits(d);
-  if (ws_bytes < kv_cache4_attention_workspace(d) || (p.splits > 1 && !ws))
-    return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
+  const size_t need = kv_cache4_attention_workspace(d);
+  if (need && (!ws || ws_bytes < need)) return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
   bind_workspace(p, ws);
   p.q_vec = aligned16(d.q, d.q_strides, d.cache.D);
   rc = run_split_attention(p, d.dtype, true, st);
-  return rc || p.splits == 1 ? rc : join(p, d.dtype, st);
+  return rc || p.splits == 1 || p.cluster ? rc : join(p, d.dtype, st);
 }
 
 }  // namespace mt

@@ -30,6 +30,7 @@ struct AttnParams {
   // split keys: partial results in the workspace
   int splits;
   int q_vec;        // 8 channels of q are one aligned 16-byte vector (attn_split_kernel)
+  int cluster;      // the splits of a row tile are a cluster and join there (attn_split_kernel)
   int target;       // CTAs that the work is cut into (attn_split_kernel)
   float2* part_ml;  // [split][B * Hkv * rows] (maximum in base 2, sum)
   float* part_o;    // [split][B * Hkv * rows][D], not divided by the sum
@@ -80,6 +81,7 @@ __device__ __forceinline__ BlockList block_list(const AttnParams& p, const SeqPo
 
 // window_attention_split.cu: few query rows over 16-bit keys (16-byte aligned rows) or the 4-bit cache
 int split_count(int64_t bk, int64_t rows, int64_t keys);
+bool split_joins_in_cluster(int64_t bk, int64_t rows, int splits);  // no workspace and no join launch then
 int run_split_attention(AttnParams& p, int dtype, bool paged, cudaStream_t st);
 
 // window_attention_sm100.cu: many queries over 16-bit keys, head dims up to 128

@@ -4,9 +4,9 @@
 // The products run on mma.m16n8k16 with the KEYS on the 16-row side and up to 8 * NT query rows on the
 // 8-column side: S^T = K Q^T, then O^T = V^T P^T.  The work is bound by reading K and V (a decoder's step
 // has 1 to 16 rows a key head), so the tensor cores only have to keep the arithmetic out of the way; with
-// the keys on the M side a fragment of K or V is exactly what a lane loads from memory, 16 bytes (or 8 / 4
-// bytes of codes) at a time, with no shared memory between: the k order of a product is free, and the
-// codes are unpacked into fragments with one shift and one logic instruction per pair.
+// the keys on the M side a fragment of K or V is what a lane reads from its warp's ring (cp.async, no
+// barrier between warps), 16 bytes or 8 / 4 bytes of codes at a time: the k order of a product is free, and
+// the codes are unpacked into fragments with one shift and one logic instruction per pair.
 //
 // Codes as operands: the 4 bits of a code at the low end of a 16-bit lane ARE the number c * 2^-133 in
 // bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly; at bits 4..7 they are 16 times that.  One
@@ -28,7 +28,8 @@ namespace mt {
 
 constexpr int kSplitWarps = 4;
 constexpr float kSplitLazy = 8.0f;
-constexpr int kMinChunk = 16;  // blocks of 16 keys that a CTA takes at least
+constexpr int kMinChunk = 16;     // blocks of 16 keys that a CTA takes at least
+constexpr int kSplitCluster = 8;  // up to so many chunks are joined within a cluster
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;
@@ -112,8 +113,9 @@ struct SplitRing {
 };
 
 // One CTA: kSplitWarps warps over one chunk of the steps (KB blocks of 16 keys, of one page) of (b, hk) for
-// 8 * NT query rows.  DC: blocks of 64 channels.  In a lane, n = lane / 4 and t = lane % 4.
-template <bool F16, bool PAGED, int DC, int NT, int KB>
+// 8 * NT query rows.  DC: blocks of 64 channels.  CLUSTER: the chunks of a row tile are a cluster, which joins them (a
+// variant of its own: the code costs registers).  In a lane, n = lane / 4 and t = lane % 4.
+template <bool F16, bool PAGED, int DC, int NT, int KB, bool CLUSTER>
 __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 2) : 1) attn_split_kernel(const AttnParams p) {
   using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
   constexpr int ROWS = 8 * NT;
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
   __shared__ float2 sml[kSplitWarps][ROWS];
   __shared__ RowKeys srk[ROWS];
   __shared__ float sinv[ROWS];
+  __shared__ float2 sfin[ROWS];  // maximum and sum of the CTA's share
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
   const int bk = blockIdx.y, b = bk / p.Hkv, hk = bk % p.Hkv;
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
   }
   const int i0 = (int)min((int64_t)blockIdx.x * per, (int64_t)bl.count), i1 = min(bl.count, i0 + per);
   const int64_t out_row = ((int64_t)blockIdx.x * p.B * p.Hkv + bk) * p.rows + r0;
-  if (i0 >= i1 && gridDim.x > 1) {
+  if (i0 >= i1 && gridDim.x > 1 && !CLUSTER) {
     if (threadIdx.x < nr) p.part_ml[out_row + threadIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
@@ -598,7 +601,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w)
       if (sml[w][r].x != -INFINITY) ls = fmaf(sml[w][r].y, ex2f(sml[w][r].x - top), ls);
-    if (gridDim.x > 1) p.part_ml[out_row + r] = make_float2(top, ls);
+    if (CLUSTER) sfin[r] = make_float2(top, ls);
+    if (gridDim.x > 1 && !CLUSTER) p.part_ml[out_row + r] = make_float2(top, ls);
     sinv[r] = ls > 0.f ? 1.f / ls : 0.f;
   }
   __syncwarp();
@@ -623,6 +627,65 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         dst[1] = make_float4(v[4], v[5], v[6], v[7]);
       }
   __syncthreads();
+  if constexpr (CLUSTER) {
+    // each CTA adds up its warps, then takes its part of the outputs over all the CTAs' sums in their shared memory,
+    // which saves the join's launch (4 tokens on 1000 keys of 4 heads of codes: 12.4 -> 10.7 us)
+    constexpr int U = ROWS * DP / 4 / (kSplitWarps * 32);
+    float4 own[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + u * kSplitWarps * 32, r = i / (DP / 4), d = i % (DP / 4) * 4;
+      own[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kSplitWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(split_smem + w * Ring::BYTES) + r * (DP + 4) + d);
+        own[u] = make_float4(own[u].x + y.x, own[u].y + y.y, own[u].z + y.z, own[u].w + y.w);
+      }
+    }
+    __syncthreads();
+    float* sum = reinterpret_cast<float*>(split_smem);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + u * kSplitWarps * 32;
+      *reinterpret_cast<float4*>(sum + i / (DP / 4) * (DP + 4) + i % (DP / 4) * 4) = own[u];
+    }
+    cluster_sync();
+    const int n_cta = gridDim.x;
+    for (int i = blockIdx.x * kSplitWarps * 32 + threadIdx.x; i < nr * (DP / 4); i += n_cta * kSplitWarps * 32) {
+      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+      float2 ml[kSplitCluster];
+      float top = -INFINITY, ls = 0.f;
+#pragma unroll
+      for (int c = 0; c < kSplitCluster; ++c) {
+        ml[c] = make_float2(-INFINITY, 0.f);
+        if (c < n_cta) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[c].x), "=f"(ml[c].y) : "r"(mapa_rank(&sfin[r], c)) : "memory");
+        top = fmaxf(top, ml[c].x);
+      }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < kSplitCluster; ++c) {
+        if (ml[c].x == -INFINITY) continue;  // (a chunk that saw nothing)
+        const float f = ex2f(ml[c].x - top);
+        float4 y;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                     : "r"(mapa_rank(sum + r * (DP + 4) + d, c))
+                     : "memory");
+        ls = fmaf(ml[c].y, f, ls);
+        x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+      }
+      if (d >= p.D) continue;  // D is a multiple of 8
+      const float inv = ls > 0.f ? 1.f / ls : 0.f;
+      const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
+      T* dst = static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + qi * p.os[2];
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[(d + j) * p.os[3]] = from_f32<T>(v[j] * inv);
+    }
+    __syncwarp();
+    cluster_sync();  // the sums stay until everybody has read them
+    return;
+  }
   for (int i = threadIdx.x; i < nr * (DP / 4); i += kSplitWarps * 32) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -652,6 +715,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
 // Query rows a key head that the split kernel takes (more rows: the tiled kernels read K and V less often).
 int split_tile_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 
+// A grid of at most two CTAs an SM, all resident at once, is joined in clusters; larger ones in a launch of their own: a
+// cluster starts when all its CTAs have room, and those without keys hold theirs until it ends.  Join's launch, cluster at
+// 2000 keys, 8 key heads of 128 channels, 16-bit rows, 1, 4, 12, 40 sequences: 10.4, 12.4, 25, 54 us against 10.4, 12.4,
+// 35, 147; codes of 64 channels, 1, 2, 4, 12, 40: 8.5, 9.8, 10.4, 14.9, 31 against 8.3, 8.6, 9.9, 16.9, 41.
+bool split_joins_in_cluster(int64_t bk, int64_t rows, int splits) {
+  const int tr = split_tile_rows(rows);
+  return splits > 1 && splits <= kSplitCluster && bk * ((rows + tr - 1) / tr) * splits <= 2 * num_sms();
+}
+
 int split_count(int64_t bk, int64_t rows, int64_t keys) {
   const int tr = split_tile_rows(rows);
   const int64_t ctas = bk * ((rows + tr - 1) / tr);
@@ -661,10 +733,10 @@ int split_count(int64_t bk, int64_t rows, int64_t keys) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 512));
 }
 
-template <bool F16, bool PAGED, int DC, int NT, int KB>
-static int split_launch_kernel(AttnParams& p, dim3 grid, cudaStream_t st) {
+template <bool F16, bool PAGED, int DC, int NT, int KB, bool CLUSTER>
+static int split_launch_cluster(AttnParams& p, dim3 grid, cudaStream_t st) {
   constexpr int smem = kSplitWarps * SplitRing<PAGED, DC, KB>::BYTES;
-  auto kern = attn_split_kernel<F16, PAGED, DC, NT, KB>;
+  auto kern = attn_split_kernel<F16, PAGED, DC, NT, KB, CLUSTER>;
   static int resident[64] = {};  // CTAs an SM holds
   int dev = 0;
   cudaGetDevice(&dev);
@@ -683,8 +755,29 @@ static int split_launch_kernel(AttnParams& p, dim3 grid, cudaStream_t st) {
   // rows, where a chunk's start costs more: 24 sequences of 4096..16384 codes take 111, 83, 83, 79, 80 us with 2, 3,
   // 8, 12, 16 CTAs an SM (4 resident), 8 sequences of 4096 16-bit keys 33, 32, 35, 37 with 2, 3, 4, 8 (2 resident)
   p.target = num_sms() * (PAGED ? 3 * res : (3 * res + 1) / 2);
-  kern<<<grid, kSplitWarps * 32, smem, st>>>(p);
-  return check_launch("attention_split");
+  if (!CLUSTER) {
+    kern<<<grid, kSplitWarps * 32, smem, st>>>(p);
+    return check_launch("attention_split");
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kSplitWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = grid.x;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  int rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, (const AttnParams)p), "attention_split");
+  return rc ? rc : check_launch("attention_split");
+}
+
+template <bool F16, bool PAGED, int DC, int NT, int KB>
+static int split_launch_kernel(AttnParams& p, dim3 grid, cudaStream_t st) {
+  return p.cluster ? split_launch_cluster<F16, PAGED, DC, NT, KB, true>(p, grid, st)
+                   : split_launch_cluster<F16, PAGED, DC, NT, KB, false>(p, grid, st);
 }
 
 template <bool F16, bool PAGED, int DC>
@@ -716,6 +809,7 @@ static int split_launch(AttnParams& p, cudaStream_t st) {
 }
 
 int run_split_attention(AttnParams& p, int dtype, bool paged, cudaStream_t st) {
+  p.cluster = split_joins_in_cluster((int64_t)p.B * p.Hkv, p.rows, p.splits);
   if (paged && ((int64_t)p.num_pages * p.Hkv << (p.page_shift - 4)) >= 0xffffffffLL)
     return fail(MT_ERR_UNSUPPORTED, "kv_cache4_attention: more than 2^36 tokens and heads in the cache");
   if (dtype == MT_F16) return paged ? split_launch<true, true>(p, st) : split_launch<true, false>(p, st);

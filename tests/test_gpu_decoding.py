@@ -469,6 +469,35 @@ def test_cache_attention_reads_no_pages_outside_the_window():
     np.testing.assert_allclose(host(got), want, rtol=2.0 ** -8, atol=(2.0 ** -8 + 1e-4) * 10)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Sq", [(2, 1), (6, 2), (10, 3)])
+@pytest.mark.parametrize("per,D", [(5, 64), (14, 128), (23, 192), (32, 256), (40, 128)])
+def test_few_sequences_over_several_chunks_of_keys(per, D, H, Sq, dtype):
+    """2 to 9 and more chunks a sequence, of which short sequences leave some or all empty; one call's bits are the next's."""
+    rng = np.random.default_rng(per + H)
+    B, Hkv, page = 3, 2, 64
+    cap = per * page
+    lengths = np.array([cap - 7, 0, Sq + 19])
+    cache, table, kq, vq = filled_cache(rng, B, Hkv, page, per, D)
+    q, qv = heads(rng, B, H, Sq, D, dtype)
+    for window, sinks in ((None, 0), (cap // 2, 9)):
+        got = mt.kv_cache_attention(q, cache, i32(table), i32(lengths), window=window, sinks=sinks)
+        want = attention_ref(qv, kq, vq, lengths - Sq, lengths, window, sinks, True)
+        np.testing.assert_allclose(host(got), want, rtol=2 * U[dtype], atol=(2.0 ** -8 + 1e-4) * max(np.abs(vq).max(), 5))
+        again = mt.kv_cache_attention(q, cache, i32(table), i32(lengths), window=window, sinks=sinks)
+        np.testing.assert_array_equal(host(got), host(again))
+    d = D - 24 if D < 256 else D  # channels that end inside a block of 64
+    q, qv = heads(rng, B, H, Sq, d, dtype)
+    k, kv = heads(rng, B, Hkv, cap, d, dtype)
+    v, vv = heads(rng, B, Hkv, cap, d, dtype)
+    for window, sinks in ((cap, 0), (cap // 2, 9)):
+        got = mt.window_attention(q, k, v, window, sinks, starts=i32(lengths - Sq), lengths=i32(lengths))
+        want = attention_ref(qv, kv, vv, lengths - Sq, lengths, window, sinks, True)
+        attention_close(got, want, dtype, 5.0)
+        again = mt.window_attention(q, k, v, window, sinks, starts=i32(lengths - Sq), lengths=i32(lengths))
+        np.testing.assert_array_equal(host(got), host(again))
+
+
 # ---------------------------------------------------------------------------------------------
 # 4-bit weights
 
