@@ -7,10 +7,11 @@
 // on the 8-column side.  Bound by reading W, and next by unpacking it: a lane's 16 bytes are words t, t + 4, t + 8,
 // t + 12 of a block of 128 columns, which are its fragments for 8 products of 16 columns.  A code's 4 bits at the low
 // end of a 16-bit lane are the number c * 2^-133 in bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly,
-// at bits 4..7 sixteen times that: one AND makes two operands, one shift serves half a word.  X is laid out once
-// per CTA as operands in shared memory, scaled to match (bf16 by 2^64; channels at bits 4..7 by another 1/16), with
-// the sums of 8 x per row and group beside it, which take the codes' offset off: y += scale (acc - sum 8 x), in fp32
-// per group of columns.  A warp brings its blocks of W with its own cp.async into a ring; no barrier stands between
+// at bits 4..7 sixteen times that: one AND makes two operands, one shift serves half a word.  The two places have
+// sums of their own (a sixteenth put on X instead would cost f16 values below 2^-10 their last bits).  X is laid out once
+// per CTA as operands in shared memory (bf16 times 2^64, to stay clear of fp32's subnormals), with the sums of -8 x
+// per row and group beside it, which take the codes' offset off: y += scale (low - 8 sum x + high / 16), in fp32 per
+// group of columns.  A warp brings its blocks of W with its own cp.async into a ring; no barrier stands between
 // the warps but at the end of a tile.
 //
 // fp32 X goes as three bf16 parts (8 + 8 + 8 bits) in three rows of their own, added at the end.
@@ -62,7 +63,6 @@ __device__ __forceinline__ void w4_mma_zero(float (&d)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-
 // Rows of the products that one row of X becomes.
 template <typename T> constexpr int w4_parts() { return sizeof(T) == 4 ? 3 : 1; }
 
@@ -72,9 +72,8 @@ __device__ __forceinline__ constexpr float w4_unit() {
   return std::is_same<T, __half>::value ? 16777216.f : 590295810358705651712.f;  // 2^24, 2^69
 }
 
-// Eight columns of X as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7), scaled as the codes' places ask; bf16 exactly,
-// f16 but for what a sixteenth of values below 2^-10 loses (at most 2^-21).  `part`: which of the three bf16 parts of
-// fp32.  Returns 8 times the columns' sum in the operands' unit.
+// Eight columns of X as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7); bf16 times 2^64, f16 as it is.  `part`: which of the three bf16 parts of
+// fp32.  Returns -8 times the columns' sum in the operands' unit.
 template <typename T>
 __device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], int part, uint4& out) {
   constexpr bool F16 = std::is_same<T, __half>::value;
@@ -87,21 +86,18 @@ __device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], 
     w[1] = __byte_perm(r.x, r.z, 0x7632);
     w[2] = __byte_perm(r.y, r.w, 0x5410);
     w[3] = __byte_perm(r.y, r.w, 0x7632);
+    if (!F16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (F16) {
-        __half2& v = *reinterpret_cast<__half2*>(&w[j]);
-        if (j & 1) v = __hmul2(v, __half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00)));  // 1/16
-      } else {
+      for (int j = 0; j < 4; ++j) {
         __nv_bfloat162& v = *reinterpret_cast<__nv_bfloat162*>(&w[j]);
-        const __nv_bfloat16 f = __ushort_as_bfloat16(j & 1 ? 0x5d80 : 0x5f80);  // 2^60, 2^64
+        const __nv_bfloat16 f = __ushort_as_bfloat16(0x5f80);  // 2^64
         v = __hmul2(v, __nv_bfloat162(f, f));
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum += to_f32<T>(e[j]);
   } else {
-    constexpr float even = 18446744073709551616.f, odd = even / 16.f;  // 2^64, 2^60
+    constexpr float f = 18446744073709551616.f;  // 2^64
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -112,10 +108,10 @@ __device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], 
       sum += v[j];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(v[j] * (j & 1 ? odd : even), v[j + 4] * (j & 1 ? odd : even));
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(v[j] * f, v[j + 4] * f);
   }
   out = make_uint4(w[0], w[1], w[2], w[3]);
-  return sum * (8.f / w4_unit<T>());
+  return sum * (-8.f / w4_unit<T>());
 }
 
 // 16 bytes to shared memory
@@ -123,7 +119,7 @@ __device__ __forceinline__ void w4_cp_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// Shared memory of a CTA for `rows` operand rows: the warps' sums, the rings, X's operands, the sums of 8 x.
+// Shared memory of a CTA for `rows` operand rows: the warps' sums, the rings, X's operands, the sums of -8 x.
 template <int GROUP, int MT, int NT, int WARPS>
 struct W4Smem {
   static constexpr int STAGES = 3;
@@ -279,22 +275,25 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const uint4 c0 = *reinterpret_cast<const uint4*>(st + i * 1024), c1 = *reinterpret_cast<const uint4*>(st + i * 1024 + 512);
-        float acc[NT][4];
+        // sums over the codes at bits 0..3, and 16 times those over the codes at bits 4..7 (one chain for both, the
+        // second divided before the first start, saves the additions and takes 36.3 us for 34.9 at 8192 -> 28672, one row)
+        float lo[NT][4], hi[NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // 32 columns
           const bool fresh = (j * 32) % GROUP == 0;
-          uint32_t w0 = j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w;
-          uint32_t w1 = j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w;
+          const uint32_t w0 = j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w, v0 = w0 >> 8;
+          const uint32_t w1 = j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w, v1 = w1 >> 8;
+          const uint32_t al[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu, v1 & 0x000f000fu};
+          const uint32_t ah[4] = {w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u, v1 & 0x00f000f0u};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-              if (fresh && e == 0) w4_mma_zero<F16>(acc[x], a, xb[j][x].x, xb[j][x].y);
-              else w4_mma<F16>(acc[x], a, e ? xb[j][x].z : xb[j][x].x, e ? xb[j][x].w : xb[j][x].y);
+          for (int x = 0; x < NT; ++x) {
+            if (fresh) {
+              w4_mma_zero<F16>(lo[x], al, xb[j][x].x, xb[j][x].z);
+              w4_mma_zero<F16>(hi[x], ah, xb[j][x].y, xb[j][x].w);
+            } else {
+              w4_mma<F16>(lo[x], al, xb[j][x].x, xb[j][x].z);
+              w4_mma<F16>(hi[x], ah, xb[j][x].y, xb[j][x].w);
             }
-            w0 >>= 8;
-            w1 >>= 8;
           }
           if ((j * 32 + 32) % GROUP == 0) {
             const int g = j * 32 / GROUP;
@@ -304,8 +303,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
               const float s = __uint_as_float(g & 1 ? w & 0xffff0000u : w << 16);
 #pragma unroll
               for (int x = 0; x < NT; ++x) {
-                y[i][x][2 * h] = fmaf(s, acc[x][2 * h] - s8[g][x].x, y[i][x][2 * h]);
-                y[i][x][2 * h + 1] = fmaf(s, acc[x][2 * h + 1] - s8[g][x].y, y[i][x][2 * h + 1]);
+                y[i][x][2 * h] = fmaf(s, fmaf(hi[x][2 * h], 0.0625f, lo[x][2 * h] + s8[g][x].x), y[i][x][2 * h]);
+                y[i][x][2 * h + 1] = fmaf(s, fmaf(hi[x][2 * h + 1], 0.0625f, lo[x][2 * h + 1] + s8[g][x].y), y[i][x][2 * h + 1]);
               }
             }
           }

@@ -531,6 +531,22 @@ def test_linear_weight4(M, N, K, group, dtype):
         assert (err <= linear_bound(xv, back, dtype, y) + 2.0 ** -22 * np.abs(add)).all(), err.max()
 
 
+@pytest.mark.parametrize("dtype,power", [("float16", -11), ("float16", -16), ("float16", -22), ("float16", 9),
+                                         ("bfloat16", -40), ("bfloat16", 40), ("float32", -40), ("float32", 40)])
+@pytest.mark.parametrize("M", [1, 13])
+def test_linear_weight4_of_small_and_large_rows(M, dtype, power):
+    """Rows whose values all lie near 2^power (f16: down to its subnormals) lose nothing to the operands' scaling."""
+    rng = np.random.default_rng(power & 63)
+    N, K = 70, 96
+    p = mt.Weight4.pack(dev(rng.standard_normal((N, K)) * 2.0 ** (-power // 2), "float32"), 32)
+    w = host(p.unpack("float32"))
+    x, xv = rounded(rng.standard_normal((M, K)) * 2.0 ** power, dtype)
+    y = xv @ w.T
+    err = np.abs(host(mt.linear_weight4(x, p)) - y)
+    floor = 2.0 ** -25 if dtype == "float16" else 0  # half of f16's smallest number
+    assert (err <= linear_bound(xv, w, dtype, y) + floor).all(), err.max()
+
+
 def test_linear_weight4_views():
     """Rows with a pitch, leading dims, out= a view, columns past K that hold anything."""
     rng = np.random.default_rng(1)
