@@ -10,7 +10,8 @@ graph) and replays it with one call (`mt_cuda_graph_launch`).
 Rules for the captured function: fixed shapes, inputs read from the static buffers created here,
 no host synchronisation inside (e.g. no `.cpu()` / `.numpy()`), and any per-weight caches
 (packed conv weights, interleaved GEGLU weights) already built — the constructor runs the
-function twice before capturing, which also sizes the shared kernel workspace.
+function twice before capturing, which also sizes the shared kernel workspace.  The graph holds the
+workspace that it was captured with: a later call that outgrows it gets another one.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ import ctypes as C
 
 from . import _lib as L
 from . import runtime
-from .tensor import Tensor
+from .tensor import _WS, Tensor
 
 
 class Graphed:
@@ -34,12 +35,14 @@ class Graphed:
         self._graph = None
         n0 = lib.mt_cuda_launch_count()
         L.check(lib.mt_cuda_graph_begin(self.stream), "graph capture begin")
-        runtime.capturing.add(self.device)
+        # the captured launches keep the workspace's address, so the buffer stays as long as the graph does
+        self._workspaces = runtime.capturing[self.device] = []
         g = C.c_void_p()
         try:
             self.static_out = fn(*self.static_in)
         finally:
-            runtime.capturing.discard(self.device)
+            runtime.capturing.pop(self.device, None)
+            self._workspaces.append(_WS.get(self.device))
             rc = lib.mt_cuda_graph_end(self.stream, C.byref(g))
         L.check(rc, "graph capture end")
         self._graph = g.value

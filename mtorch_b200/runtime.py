@@ -23,7 +23,7 @@ from . import _lib as L
 _current = [0]
 _initialised: set = set()
 _streams: dict = {}
-capturing: set = set()  # devices with a graph capture open (graphs.Graphed)
+capturing: dict = {}  # device with a graph capture open -> workspaces outgrown during it (graphs.Graphed)
 
 
 def _ensure_device(idx: int) -> None:

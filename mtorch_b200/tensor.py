@@ -128,17 +128,17 @@ def _alloc(nbytes: int, idx: int) -> DeviceBuffer:
 
 
 _WS: dict = {}
-_WS_RETIRED: list = []
 
 
 def workspace(nbytes: int, idx: int):
-    """Per-device scratch buffer handed to the kernels (grown on demand, reused in stream order)."""
+    """Per-device scratch buffer handed to the kernels (grown on demand, reused in stream order).  A captured graph's
+    launches keep its address: `graphs.Graphed` holds the buffers that its capture used."""
     if nbytes <= 0:
         return None, 0
     buf = _WS.get(idx)
     if buf is None or buf.numel() < nbytes:
         if buf is not None and idx in _rt.capturing:
-            _WS_RETIRED.append(buf)  # kernels captured earlier in this graph still use it
+            _rt.capturing[idx].append(buf)  # kernels captured earlier in this graph still use it
         buf = _alloc(int(nbytes * 1.25) + 4096, idx)
         _WS[idx] = buf
     return buf.data_ptr(), buf.numel()
