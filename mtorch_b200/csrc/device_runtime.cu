@@ -85,18 +85,17 @@ cudaError_t raw_malloc(void** p, size_t bytes) {
   return e;
 }
 
-// Releases every cached (free) block of `dev` in pools that no capture is using; g_mu held.
+// Releases every cached (free) block of `dev` in the default pool; g_mu held.  The free blocks of a graph's pool are
+// temporaries that its replays still write: they go with the graph (mt_cuda_graph_destroy).
 void release_cached(int dev) {
   DeviceState& s = g_dev[dev];
   cudaDeviceSynchronize();
-  for (size_t p = 0; p < s.pools.size(); ++p) {
-    if ((int)p == s.active_pool && p != 0) continue;
-    for (auto& kv : s.pools[p].free_blocks) {
-      cudaFree(kv.second);
-      s.cached -= kv.first;
-    }
-    s.pools[p].free_blocks.clear();
+  Pool& pool = s.pools[0];
+  for (auto& kv : pool.free_blocks) {
+    cudaFree(kv.second);
+    s.cached -= kv.first;
   }
+  pool.free_blocks.clear();
 }
 
 }  // namespace

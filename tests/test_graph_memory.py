@@ -106,3 +106,26 @@ def test_replay_after_the_workspace_grew():
     assert all(t.data_ptr() + size <= lo or t.data_ptr() >= hi for t in others)
     np.testing.assert_array_equal(g(q).float().numpy(), want)
     assert all((t.float().numpy() == 0).all() for t in others)
+
+
+@pytest.mark.gpu
+def test_empty_cache_leaves_a_graphs_temporaries():
+    """What a capture freed is written again by every replay: it stays until the graph is gone."""
+    rng = np.random.default_rng(2)
+    x = mt.tensor(rng.standard_normal((1024, 1024)).astype(np.float32)).to("bfloat16").cuda()
+
+    def fn(t):
+        return t * 2 + t * 3
+
+    want = fn(x).float().numpy()
+    g = graphs.Graphed(fn, x)
+    mt.cuda.empty_cache()
+    held = runtime.memory_stats(0)["cached_bytes"]
+    assert held >= 2 * x.numel() * 2  # the two products
+    others = [mt.zeros(1024, 1024, dtype="bfloat16", device="cuda") for _ in range(4)]
+    np.testing.assert_array_equal(g(x).float().numpy(), want)
+    assert all((t.float().numpy() == 0).all() for t in others)
+    del g
+    gc.collect()
+    mt.cuda.empty_cache()
+    assert runtime.memory_stats(0)["cached_bytes"] < held
