@@ -62,6 +62,13 @@ __device__ __forceinline__ uint64_t wa_add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// subnormal numbers to zero
+__device__ __forceinline__ uint64_t wa_flush2(uint64_t a) {
+  uint64_t r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(wa_pack2(1.f, 1.f)));
+  return r;
+}
+
 // maximum of 128 values, eight independent chains
 __device__ __forceinline__ float wa_max128(const uint32_t (&r)[128]) {
   float m[8];
@@ -78,7 +85,8 @@ __device__ __forceinline__ float wa_max128(const uint32_t (&r)[128]) {
 
 // 2^x of two values on the FMA pipe: x = i + f with |f| <= 1/2, a polynomial for 2^f (minimax in relative error by the
 // Remez exchange: 7.5e-5 for degree 3, 2.6e-6 for degree 4, a fraction of P's rounding to bf16 / f16), i added to
-// the exponent.  Below 2^-126 it stays there.
+// the exponent.  x at or below -126 (a hidden key's is -inf) gives 0: there the polynomial's value is just below
+// 2^-126, and the last product flushes it, so that a hidden key's V counts nothing however large it is.
 template <bool F16>
 __device__ __forceinline__ void wa_exp2_poly(float& a0, float& a1) {
   a0 = fmaxf(a0, -126.f);
@@ -103,6 +111,7 @@ __device__ __forceinline__ void wa_exp2_poly(float& a0, float& a1) {
   wa_unpack2(y, a0, a1);
   a0 = __uint_as_float(__float_as_uint(a0) + (__float_as_uint(t0) << 23));
   a1 = __uint_as_float(__float_as_uint(a1) + (__float_as_uint(t1) << 23));
+  wa_unpack2(wa_flush2(wa_pack2(a0, a1)), a0, a1);
 }
 
 // bits c of the 32 columns from `base` on that a row sees
