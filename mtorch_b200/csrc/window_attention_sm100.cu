@@ -38,9 +38,15 @@ __device__ __forceinline__ float wa_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// maxima that keep a NaN: a row with a NaN among the scores that it sees has to end as NaN
 __device__ __forceinline__ float wa_max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float wa_max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t wa_pack2(float a, float b) {
@@ -79,8 +85,8 @@ __device__ __forceinline__ float wa_max128(const uint32_t (&r)[128]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) m[i] = wa_max3(m[i], __uint_as_float(r[k + i]), __uint_as_float(r[k + 8 + i]));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], __uint_as_float(r[120 + i]));
-  return wa_max3(wa_max3(m[0], m[1], m[2]), wa_max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+  for (int i = 0; i < 8; ++i) m[i] = wa_max2(m[i], __uint_as_float(r[120 + i]));
+  return wa_max3(wa_max3(m[0], m[1], m[2]), wa_max3(m[3], m[4], m[5]), wa_max2(m[6], m[7]));
 }
 
 // 2^x of two values on the FMA pipe: x = i + f with |f| <= 1/2, a polynomial for 2^f (minimax in relative error by the
@@ -439,8 +445,11 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         }
       }
       const float top = wa_max128(r);
-      if (__any_sync(0xffffffffu, top > thr)) {
-        const float mn = fmaxf(m, top);
+      // A NaN stays in m (the comparison with it is false), as does what infinity - infinity gives: from then on
+      // every weight of the row is NaN.  The polynomial alone would turn a NaN score into a number.
+      if (__any_sync(0xffffffffu, !(top <= thr))) {
+        float mn = wa_max2(m, top);
+        if (mn == INFINITY) mn = NAN;
         const float corr = m == -INFINITY ? 0.f : wa_ex2((m - mn) * sl);
         m = mn;
         thr = m + kWaLazy / sl;

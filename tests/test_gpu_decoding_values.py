@@ -44,3 +44,37 @@ def test_hidden_keys_count_nothing(form, dtype, H, Hkv, Sq, Sk, D):
     assert clean.any()
     want = attention_ref(qv, kv, np.where(far[:, None], 0, vv), [Sk - Sq], [Sk], window, 0, True)
     np.testing.assert_allclose(got[:, :, clean], want[:, :, clean], rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
+
+
+NAN_FORMS = [f for f in FORMS if f[0] in ("tc", "tiles")]
+
+
+@pytest.mark.parametrize("what", ["nan query", "nan key", "nan keys", "infinite score"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form,dtype,H,Hkv,Sq,Sk", NAN_FORMS)
+def test_nan_is_not_lost(form, dtype, H, Hkv, Sq, Sk, D, what):
+    """A query whose scores hold a NaN, or an infinity (whose difference with itself is one), gives NaN; others do not."""
+    rng = np.random.default_rng(Sq + D)
+    window, sinks = 90, 2
+    qn, kn = rng.standard_normal((1, H, Sq, D)), rng.standard_normal((1, Hkv, Sk, D))
+    p = Sk - Sq + np.arange(Sq)
+    qn[..., 7] = np.abs(qn[..., 7]) + 1
+    hit = np.zeros((H, Sq), bool)
+    group = np.arange(H) * Hkv // H  # key head of a head
+    if what == "nan query":
+        qn[0, 1, Sq // 2, 3] = np.nan
+        hit[1, Sq // 2] = True
+    else:
+        at = {"nan key": [242], "nan keys": list(range(Sk)), "infinite score": [243]}[what]
+        kn[0, -1, at, 7] = np.inf if what == "infinite score" else np.nan
+        sees = np.array([any(a <= i and (i - a < window or a < sinks) for a in at) for i in p])
+        hit[group == Hkv - 1] = sees
+    q, qv = rounded(qn, dtype)
+    k, kv = rounded(kn, dtype)
+    v, vv = heads(rng, 1, Hkv, Sk, D, dtype)
+    assert path_of(q, k, v, window, sinks) == form
+    got = host(mt.window_attention(q, k, v, window, sinks))[0]
+    assert np.isnan(got[hit]).all() and hit.any()
+    with np.errstate(invalid="ignore"):
+        want = attention_ref(qv, np.where(np.isfinite(kv), kv, 0), vv, [Sk - Sq], [Sk], window, sinks, True)[0]
+    np.testing.assert_allclose(got[~hit], want[~hit], rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
