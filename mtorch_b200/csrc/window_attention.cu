@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParam
     const int at = vec ? d : d * 4, step = n * 4;
     float y = 0.f;
     for (int i = 0; i < groups; ++i) y += red[i * step + at];
-    dst[d * p.os[3]] = from_f32<T>(ls > 0.f ? y / ls : 0.f);
+    dst[d * p.os[3]] = from_f32<T>(ls == 0.f ? 0.f : y / ls);
   }
 }
 

@@ -36,6 +36,13 @@ struct AttnParams {
   float* part_o;    // [split][B * Hkv * rows][D], not divided by the sum
 };
 
+// A maximum that keeps a NaN: a query whose scores hold one has to end as NaN, also where shares of its keys are joined.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Keys n and the first query's position of one batch entry.
 struct SeqPos {
   int n, start;

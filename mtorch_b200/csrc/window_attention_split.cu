@@ -430,9 +430,9 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float top = fmaxf(sc[0][x][j], sc[0][x][2 + j]);
-        if (KB == 2) top = fmaxf(top, fmaxf(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
-        over |= top > thr[x][j];
+        float top = max_nan(sc[0][x][j], sc[0][x][2 + j]);
+        if (KB == 2) top = max_nan(top, max_nan(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
+        over |= !(top <= thr[x][j]);  // (a NaN too: it stays in m, and all the weights to come are NaN)
       }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -440,12 +440,12 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         float corr[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float mx = fmaxf(sc[0][x][j], sc[0][x][2 + j]);
-          if (KB == 2) mx = fmaxf(mx, fmaxf(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[x][j]);
+          float mx = max_nan(sc[0][x][j], sc[0][x][2 + j]);
+          if (KB == 2) mx = max_nan(mx, max_nan(sc[KB - 1][x][j], sc[KB - 1][x][2 + j]));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = max_nan(mx, m[x][j]);
           corr[j] = m[x][j] == -INFINITY ? 0.f : ex2f((m[x][j] - mx) * score_scale);
           m[x][j] = mx;
           thr[x][j] = mx + kSplitLazy / score_scale;
@@ -597,13 +597,13 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     const int r = threadIdx.x;
     float top = -INFINITY, ls = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, sml[w][r].x);
+    for (int w = 0; w < kSplitWarps; ++w) top = max_nan(top, sml[w][r].x);
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w)
       if (sml[w][r].x != -INFINITY) ls = fmaf(sml[w][r].y, ex2f(sml[w][r].x - top), ls);
     if (CLUSTER) sfin[r] = make_float2(top, ls);
     if (gridDim.x > 1 && !CLUSTER) p.part_ml[out_row + r] = make_float2(top, ls);
-    sinv[r] = ls > 0.f ? 1.f / ls : 0.f;
+    sinv[r] = ls == 0.f ? 0.f : 1.f / ls;
   }
   __syncwarp();
   float* mine = reinterpret_cast<float*>(ring);
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
       }
       if (d >= p.D) continue;  // D is a multiple of 8
-      const float inv = ls > 0.f ? 1.f / ls : 0.f;
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
       const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
       T* dst = static_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + qi * p.os[2];
       const float v[4] = {x.x, x.y, x.z, x.w};

@@ -46,7 +46,7 @@ def test_hidden_keys_count_nothing(form, dtype, H, Hkv, Sq, Sk, D):
     np.testing.assert_allclose(got[:, :, clean], want[:, :, clean], rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
 
 
-NAN_FORMS = [f for f in FORMS if f[0] in ("tc", "tiles")]
+NAN_FORMS = [f for f in FORMS if f[0] in ("tc", "split", "tiles")]
 
 
 @pytest.mark.parametrize("what", ["nan query", "nan key", "nan keys", "infinite score"])
@@ -78,3 +78,47 @@ def test_nan_is_not_lost(form, dtype, H, Hkv, Sq, Sk, D, what):
     with np.errstate(invalid="ignore"):
         want = attention_ref(qv, np.where(np.isfinite(kv), kv, 0), vv, [Sk - Sq], [Sk], window, sinks, True)[0]
     np.testing.assert_allclose(got[~hit], want[~hit], rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
+
+
+def filled(rng, B, Hkv, page, per, D):
+    """A cache of random keys and values and what it holds, read back: [B, Hkv, page * per, D]."""
+    cache = mt.KVCache4.empty(B * per, page, Hkv, D)
+    table = i32(rng.permutation(B * per).reshape(B, per))
+    k, _ = rounded(rng.standard_normal((B, Hkv, page * per, D)) + rng.standard_normal((Hkv, 1, D)), "float32")
+    v, _ = rounded(rng.standard_normal((B, Hkv, page * per, D)) + rng.standard_normal((Hkv, 1, D)), "float32")
+    zero = i32(np.zeros(B))
+    mt.kv_cache_append(cache, k, v, table, zero)
+    kq, vq = mt.kv_cache_read(cache, table, zero, page * per, dtype="float32")
+    return cache, table, host(kq), host(vq)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [(1, 4, 1, 1, 6000, 64), (1, 8, 2, 2, 900, 128), (24, 16, 8, 1, 3000, 128)])
+def test_nan_is_not_lost_in_the_join(B, H, Hkv, Sq, Sk, D, dtype):
+    """A query of NaN over keys that are split over CTAs (joined in a cluster, or by a second kernel), and a chunk of keys
+    of which all are NaN."""
+    rng = np.random.default_rng(Sk)
+    qn = rng.standard_normal((B, H, Sq, D))
+    qn[0, 1] = np.nan
+    kn = rng.standard_normal((B, Hkv, Sk, D))
+    q, qv = rounded(qn, dtype)
+    k, kv = rounded(kn, dtype)
+    v, vv = heads(rng, B, Hkv, Sk, D, dtype)
+    assert path_of(q, k, v, None, 0) == "split"
+    want = attention_ref(np.nan_to_num(qv), kv, vv, [Sk - Sq] * B, [Sk] * B, None, 0, True)
+    got = host(mt.window_attention(q, k, v, None))
+    assert np.isnan(got[0, 1]).all()
+    got[0, 1], want[0, 1] = 0, 0
+    np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
+    kn[0, 0, :Sk // 2] = np.nan
+    k, _ = rounded(kn, dtype)
+    got = host(mt.window_attention(q, k, v, None))
+    assert np.isnan(got[0, :H // Hkv]).all() and np.isfinite(got[0, max(2, H // Hkv):]).all()
+    if D % 64 == 0:
+        cache, table, kq, vq = filled(rng, B, Hkv, 64, (Sk + 63) // 64, D)
+        lengths = np.full(B, Sk)
+        got = host(mt.kv_cache_attention(q, cache, table, i32(lengths)))
+        assert np.isnan(got[0, 1]).all()
+        want = attention_ref(np.nan_to_num(qv), kq, vq, lengths - Sq, lengths, None, 0, True)
+        got[0, 1], want[0, 1] = 0, 0
+        np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(2.0 ** -8 + 1e-4) * 8)
