@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
 #pragma unroll
         for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
         if (!live || !rk[r].sees(key)) continue;
-        const float mn = fmaxf(m[r], s);
+        // a NaN stays in m and makes the row's weights NaN
+        const float mn = max_nan(m[r], s);
         const float corr = exp2f(m[r] - mn), e = exp2f(s - mn);
         m[r] = mn;
         l[r] = fmaf(l[r], corr, e);
@@ -121,8 +122,8 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
   // join the four key groups of the warp, then the four warps
 #pragma unroll
   for (int r = 0; r < kRowTile; ++r) {
-    float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    float top = max_nan(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
     const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
     float ls = l[r] * f;
     ls += __shfl_xor_sync(0xffffffffu, ls, 8);
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
     if (d >= p.D) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][r].x);
+    for (int w = 0; w < 4; ++w) top = max_nan(top, sml[w][r].x);
     float ls = 0.f, x = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
     } else {
       const int qi = (r0 + r) / p.g, h = hk * p.g + (r0 + r) % p.g;
       static_cast<T*>(p.o)[b * p.os[0] + h * p.os[1] + qi * p.os[2] + d * p.os[3]] =
-          from_f32<T>(ls > 0.f ? x / ls : 0.f);
+          from_f32<T>(ls == 0.f ? 0.f : x / ls);
     }
   }
 }
