@@ -106,9 +106,9 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnParams p) {
 #pragma unroll
         for (int x = 1; x < 8; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
         if (!live || !rk[r].sees(key)) continue;
-        // a NaN stays in m and makes the row's weights NaN
+        // a score of -infinity weighs nothing, also as the first one; a NaN stays in m and makes the row's weights NaN
         const float mn = max_nan(m[r], s);
-        const float corr = exp2f(m[r] - mn), e = exp2f(s - mn);
+        const float corr = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn), e = s == -INFINITY ? 0.f : exp2f(s - mn);
         m[r] = mn;
         l[r] = fmaf(l[r], corr, e);
 #pragma unroll

@@ -77,6 +77,28 @@ def test_nan_is_not_lost(form, dtype, H, Hkv, Sq, Sk, D, what):
     np.testing.assert_allclose(got[~hit], want[~hit], rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form,dtype,H,Hkv,Sq,Sk", FORMS)
+def test_scores_of_minus_infinity_weigh_nothing(form, dtype, H, Hkv, Sq, Sk, D):
+    """Keys whose scores are -infinity count as hidden ones, the first that a query sees among them; a query that sees no
+    others gets zeros."""
+    rng = np.random.default_rng(Sq + D)
+    window = 30
+    qn, kn = rng.standard_normal((1, H, Sq, D)), rng.standard_normal((1, Hkv, Sk, D))
+    qn[..., 5] = np.abs(qn[..., 5]) + 1
+    gone = np.zeros(Sk, bool)
+    gone[[0, 1, 100]] = gone[Sk - 5:Sk - 2] = gone[Sk - 34:Sk - 20] = True
+    kn[:, :, gone, 5] = -np.inf
+    q, qv = rounded(qn, dtype)
+    k, kv = rounded(kn, dtype)
+    v, vv = heads(rng, 1, Hkv, Sk, D, dtype)
+    assert path_of(q, k, v, window, 0) == form
+    got = host(mt.window_attention(q, k, v, window, 0))
+    want = attention_ref(qv, kv, vv, [Sk - Sq], [Sk], window, 0, True)
+    assert Sq < Sk or (want[:, :, :2] == 0).all()
+    np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(2 * U[dtype] + 1e-4) * 5)
+
+
 def filled(rng, B, Hkv, page, per, D):
     """A cache of random keys and values and what it holds, read back: [B, Hkv, page * per, D]."""
     cache = mt.KVCache4.empty(B * per, page, Hkv, D)
