@@ -444,7 +444,8 @@ typedef struct {
 } mt_kv_cache4;
 /* Writes T tokens per sequence at positions starts[b] .. starts[b] + T - 1 (positions below 0 or
  * past the table are not written).  Per 64 channels, in fp32: zero = f16(min), scale =
- * f16((max - min) * (1/15)) (both clamped to the f16 range), code = clamp(rint((x - zero) / scale), 0, 15). */
+ * f16((max - min) * (1/15)) (both clamped to the f16 range), code = clamp(rint((x - zero) / scale), 0, 15).
+ * A NaN among the 64, or one infinity in all of them, makes the scale NaN: they read back as NaN. */
 int mt_cuda_kv_cache4_append(const mt_kv_cache4* cache, const void* k, const int64_t* k_strides, const void* v,
                              const int64_t* v_strides, int dtype, int64_t B, int64_t T, const int32_t* block_table,
                              int64_t table_stride, int64_t max_pages, const int32_t* starts, void* stream);

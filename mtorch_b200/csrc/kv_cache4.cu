@@ -65,7 +65,20 @@ __device__ __forceinline__ Vec8<T> load8(const T* src, int64_t st, bool vec) {
 
 constexpr int kAppendTokens = 1, kReadTokens = 4;  // consecutive tokens of a thread
 
+// minimum and maximum that keep a NaN
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // The code word and (scale, zero) of eight channels of a group of 64, whose other channels neighbouring lanes hold.
+// A NaN in the group makes its scale and zero NaN, as does a group of one infinity only (max - min): it reads back as NaN.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const Vec8<T>& in, __half2& scale_zero) {
   float x[8];
@@ -74,16 +87,16 @@ __device__ __forceinline__ uint32_t quantise8(const Vec8<T>& in, __half2& scale_
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int j = 1; j < 8; ++j) {
-    lo = fminf(lo, x[j]);
-    hi = fmaxf(hi, x[j]);
+    lo = min_nan(lo, x[j]);
+    hi = max_nan(hi, x[j]);
   }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const __half zero = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  const __half scale = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
+  const __half zero = __float2half_rn(min_nan(max_nan(lo, -65504.f), 65504.f));
+  const __half scale = __float2half_rn(min_nan(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.f));
   scale_zero = __halves2half2(scale, zero);
   const float z = __half2float(zero), s = __half2float(scale);
   // code = clamp(rint((x - z) / s), 0, 15), ties to the even code.  The quotient by a multiplication is within 2^-22 of

@@ -272,7 +272,8 @@ def _cache_move(cache, k, v, table, starts, T, fn, what):
 def kv_cache_append(cache: KVCache4, k: Tensor, v: Tensor, block_table: Tensor, starts: Tensor) -> None:
     """Writes `k` and `v` [B, heads, T, dim] to the cache as tokens starts[b] .. starts[b] + T - 1 of each
     sequence.  Per 64 channels (fp32): zero = f16(min), scale = f16((max - min) / 15), code =
-    clamp(round((x - zero) / scale), 0, 15).  Tokens without a page in the table are not written."""
+    clamp(round((x - zero) / scale), 0, 15); a NaN makes its 64 channels NaN.  Tokens without a page in the table are
+    not written."""
     what = "kv_cache_append"
     _require_cuda(k, v, block_table, starts)
     if k.dim() != 4:

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import mtorch_b200 as mt
-from test_gpu_decoding import U, attention_close, attention_ref, heads, host, i32, path_of, rounded
+from test_gpu_decoding import U, attention_ref, heads, host, i32, path_of, quantised, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +141,37 @@ def test_nan_is_not_lost_in_the_join(B, H, Hkv, Sq, Sk, D, dtype):
         want = attention_ref(np.nan_to_num(qv), kq, vq, lengths - Sq, lengths, None, 0, True)
         got[0, 1], want[0, 1] = 0, 0
         np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(2.0 ** -8 + 1e-4) * 8)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_cache_keeps_nan_and_infinities(dtype):
+    """Groups with a NaN, of NaN only, with infinities of one or both signs, of one infinity only, next to clean ones; a
+    sequence that sees such keys gives NaN, another does not."""
+    rng = np.random.default_rng(11)
+    B, H, T, D = 2, 2, 40, 128
+    x = rng.standard_normal((2, B, H, T, D))
+    x[:, 0, 0, 3, 70] = np.nan
+    x[:, 0, 0, 4, 64:] = np.nan
+    x[:, 0, 1, 5, 9] = np.inf
+    x[:, 0, 1, 6, 10] = -np.inf
+    x[:, 0, 1, 7, [11, 60]] = [-np.inf, np.inf]
+    x[:, 0, 1, 8, :64] = np.inf
+    x[:, 0, 1, 9, :64] = -np.inf
+    cache = mt.KVCache4.empty(2 * B, 32, H, D)
+    table, zero = i32([[3, 1], [0, 2]]), i32([0, 0])
+    k, kv = rounded(x[0], dtype)
+    v, vv = rounded(x[1], dtype)
+    mt.kv_cache_append(cache, k, v, table, zero)
+    got = mt.kv_cache_read(cache, table, zero, T, dtype="float32")
+    for g, a in zip(got, (kv, vv)):
+        with np.errstate(invalid="ignore"):
+            want = quantised(a)
+        assert np.isnan(want[0, 0, 3, 64:]).all() and np.isnan(want[0, 1, 8, :64]).all() and np.isfinite(want[1]).all()
+        np.testing.assert_allclose(host(g), want, rtol=2.0 ** -23, atol=1e-6)
+    q, qv = heads(rng, B, 4, 1, D, "bfloat16")
+    o = host(mt.kv_cache_attention(q, cache, table, i32([T, T])))
+    assert np.isnan(o[0, :2]).all() and np.isfinite(o[1]).all()
+    o = host(mt.kv_cache_attention(q, cache, table, i32([T, T]), window=20))  # (the window is past them)
+    want = attention_ref(qv, quantised(np.nan_to_num(kv, posinf=0, neginf=0)), quantised(np.nan_to_num(vv, posinf=0, neginf=0)),
+                         [T - 1] * 2, [T] * 2, 20, 0, True)
+    np.testing.assert_allclose(o, want, rtol=2 * U["bfloat16"], atol=(2.0 ** -8 + 1e-4) * 5)
