@@ -10,8 +10,9 @@
 //
 // Codes as operands: the 4 bits of a code at the low end of a 16-bit lane ARE the number c * 2^-133 in
 // bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly; at bits 4..7 they are 16 times that.  One
-// AND makes two operands, one shift serves half a word.  bf16 queries are scaled by 2^64 (exact) to keep
-// the products far from fp32's own subnormals, their channels at bits 4..7 by 2^60.  With value = zero + scale c:
+// AND makes two operands, one shift serves half a word.  bf16 queries are multiplied by a power of two (exact), one
+// for the CTA's rows, that takes the largest finite value among them to 2^63..2^64: the products stay far from fp32's
+// own subnormals, and no value passes bf16's range.  Channels at bits 4..7 get a sixteenth.  With value = zero + scale c:
 //   q.k = scale (q.c) + zero sum(q)  per 64 channels,
 //   o   = sum (p scale) c + sum p zero,
 // with p scale rounded to bf16 (for f16 queries too, whose exponents are too few for p scale; they get the rounding's
@@ -75,6 +76,18 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int i) {
 }
 constexpr float kPow64 = 18446744073709551616.f;          // 2^64
 constexpr float kPow69 = 32.f * kPow64;                    // 2^69 = 2^133 / 2^64
+__device__ __forceinline__ float pow2f(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
+// |a| and |b|, the larger of each half; NaN is dropped
+template <bool F16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  if (F16) {
+    const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  const __nv_bfloat162 m =
+      __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
 
 // 16 bytes to shared memory, zeros when !live
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -163,10 +176,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
   const RowKeys ra = row_keys(p, sp, pmin), rz = row_keys(p, sp, pmax);
   __syncthreads();
 
-  // scores, their running maximum m and the bound `thr` past which it is raised are in units of
-  // 1 / score_scale (base 2); p = 2^(score - m + kShift)
-  constexpr float kShift = PAGED ? 64.f : 0.f;
-  const float score_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * (!PAGED ? 1.f : F16 ? 16777216.f : kPow69);
+  constexpr float kShift = PAGED ? 64.f : 0.f;  // p = 2^(score - m + kShift)
   float m[NT][2], thr[NT][2], negm[NT][2], l[NT][2], cor[NT][DC][2], o[DC][4][NT][4];
   float psum[PAGED ? DC : 1][NT][4];  // sums of the rounded weights, as a product with ones
 #pragma unroll
@@ -299,6 +309,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     }
   }
   // Q fragments (while the first keys are on their way): dense, 8 channels at 32 c + 8 t of row n; paged, the channel order of the codes' pairs
+  constexpr bool NORM = PAGED && !F16;  // rows multiplied by 2^kq
   uint32_t qf[NT][2 * DC][4];
   float qsum[NT][DC][2];
 #pragma unroll
@@ -310,8 +321,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
 #pragma unroll
     for (int c = 0; c < 2 * DC; ++c) {
       const int base = PAGED ? (c >> 1) * 64 + t * 16 + (c & 1) * 8 : c * 32 + t * 8;
-      float v[8];
-      uint16_t u[8];
       alignas(16) T raw[8];
       if (p.q_vec) {  // (D is a multiple of 8)
         *reinterpret_cast<uint4*>(raw) = live && base < p.D ? __ldg(reinterpret_cast<const uint4*>(src + base)) : make_uint4(0, 0, 0, 0);
@@ -320,11 +329,61 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         for (int j = 0; j < 8; ++j) raw[j] = live && base + j < p.D ? src[(base + j) * p.qs[3]] : from_f32<T>(0.f);
       }
 #pragma unroll
+      for (int j = 0; j < 4; ++j) qf[x][c][j] = reinterpret_cast<const uint32_t*>(raw)[j];
+    }
+  }
+  int kq = 0;
+  if (NORM) {
+    constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+    uint32_t top2 = 0;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int c = 0; c < 2 * DC; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top2 = max_abs2<F16>(top2, qf[x][c][j]);
+    uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16));
+    if (top >= kInf) {  // an infinity: the largest of the others
+      top = 0;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int c = 0; c < 2 * DC; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t u0 = qf[x][c][j] & 0x7fffu, u1 = qf[x][c][j] >> 16 & 0x7fffu;
+            top = max(top, max(u0 < kInf ? u0 : 0u, u1 < kInf ? u1 : 0u));
+          }
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    const uint16_t top16 = (uint16_t)top;
+    kq = (F16 ? 14 : 63) + 127 - (int)(__float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&top16))) >> 23);
+  }
+  const float q_up[2] = {pow2f(kq >> 1), pow2f(kq - (kq >> 1))};
+  // scores, their running maximum m and the bound `thr` past which it is raised are in units of 1 / score_scale
+  // (base 2); over codes a product counts 2^-24 (f16) or 2^-133.  Past 2^120 (queries near the end of bf16's range)
+  // it makes no difference between scores that far apart.
+  const int unit = (F16 ? 24 : 133) - kq;
+  const float score_scale =
+      !PAGED ? fmaxf(fabsf(p.scale_log2), 1e-30f)
+             : fmaxf(fminf(fabsf(p.scale_log2) * pow2f(unit >> 1) * pow2f(unit - (unit >> 1)), kPow64 * 72057594037927936.f),
+                     1.17549435e-38f);  // 2^120, 2^-126
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+#pragma unroll
+    for (int c = 0; c < 2 * DC; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = qf[x][c][j];
+      const T* raw = reinterpret_cast<const T*>(w);
+      float v[8];
+      uint16_t u[8];
+#pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = to_f32<T>(raw[j]);
         if (p.scale_log2 < 0.f) v[j] = -v[j];  // the maximum is taken of unscaled scores
-        const float f = !PAGED ? 1.f : (F16 ? 1.f : kPow64) * (j & 1 ? 0.0625f : 1.f);
-        const T h = from_f32<T>(v[j] * f);
+        if (NORM) v[j] = v[j] * q_up[0] * q_up[1];
+        const T h = from_f32<T>(PAGED && (j & 1) ? v[j] * 0.0625f : v[j]);
         u[j] = *reinterpret_cast<const uint16_t*>(&h);
       }
 #pragma unroll
@@ -334,7 +393,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += v[j];
-        s *= F16 ? 1.f / 16777216.f : 1.f / kPow69;  // the unit of q.c below
+        s *= F16 ? 1.f / 16777216.f : 1.f / kPow69 / kPow64;  // the unit of q.c below
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
@@ -342,7 +401,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
         qsum[x][c >> 1][1] = (c & 1) ? qsum[x][c >> 1][1] + s1 : s1;
       }
     }
-  }
   int stage = 0;
   for (; i < i1; i += kSplitWarps) {
     const int k0 = bl.block(i) * STEP;

@@ -175,3 +175,49 @@ def test_cache_keeps_nan_and_infinities(dtype):
     want = attention_ref(qv, quantised(np.nan_to_num(kv, posinf=0, neginf=0)), quantised(np.nan_to_num(vv, posinf=0, neginf=0)),
                          [T - 1] * 2, [T] * 2, 20, 0, True)
     np.testing.assert_allclose(o, want, rtol=2 * U["bfloat16"], atol=(2.0 ** -8 + 1e-4) * 5)
+
+
+def cache_close(got, want, dtype, vmax):
+    """Over the cache a bf16 query's weights times scale are rounded to bf16 once, 2^-9 against codes of -8..7 (8 scale in the
+    place of |v|); an f16 query's carry the rounding's rest, which leaves 2^-18.  Scores move the result by at most 1e-4
+    of |v| (fp32 sums of D products), the result is rounded to its type."""
+    weights = 2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -17
+    np.testing.assert_allclose(got, want, rtol=2 * U[dtype], atol=(weights + 1e-4) * vmax)
+
+
+@pytest.mark.parametrize("H,Hkv,Sq,D,page", [(4, 2, 1, 64, 16), (8, 2, 3, 128, 32), (2, 2, 1, 256, 16), (12, 1, 2, 64, 64)])
+@pytest.mark.parametrize("dtype,power", [("bfloat16", 64), ("bfloat16", 90), ("bfloat16", 122), ("bfloat16", -60),
+                                         ("bfloat16", -90)])
+def test_cache_attention_of_small_and_large_queries(H, Hkv, Sq, D, page, dtype, power):
+    """Queries near 2^power with a scale to match see what ordinary ones do; a head of them beside ordinary ones does too."""
+    rng = np.random.default_rng(D + abs(power))
+    B, per = 2, 6
+    cache, table, kq, vq = filled(rng, B, Hkv, page, per, D)
+    n = page * per
+    lengths = np.array([n, n - 7])
+    qn = rng.standard_normal((B, H, Sq, D)) * 2.0 ** power
+    scale = 2.0 ** -power / np.sqrt(D)
+    for mixed in (False, True):
+        if mixed:
+            qn[:, 0] *= 2.0 ** (-20 if power > 0 else 20)  # scores near 0, or far apart
+        q, qv = rounded(qn, dtype)
+        got = host(mt.kv_cache_attention(q, cache, table, i32(lengths), scale=scale))
+        want = attention_ref(qv, kq, vq, lengths - Sq, lengths, None, 0, True, scale)
+        if mixed and power < 0:
+            got, want = got[:, 1:], want[:, 1:]  # (scores of millions: one key takes all, or two are within fp32's rounding)
+        cache_close(got, want, dtype, max(np.abs(vq).max(), 5))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_cache_attention_of_an_infinite_query(dtype):
+    """It gives NaN (infinity times a value of zero, or scores of both signs) and leaves the others alone."""
+    rng = np.random.default_rng(8)
+    cache, table, kq, vq = filled(rng, 1, 2, 32, 4, 64)
+    qn = rng.standard_normal((1, 8, 2, 64))
+    qn[0, 1, 0, 9], qn[0, 6, 1, 10] = np.inf, -np.inf
+    q, qv = rounded(qn, dtype)
+    got = host(mt.kv_cache_attention(q, cache, table, i32([128])))
+    bad = ~np.isfinite(qv).all(-1)
+    assert np.isnan(got[bad]).all() and bad.sum() == 2
+    want = attention_ref(np.where(np.isfinite(qv), qv, 0), kq, vq, [126], [128], None, 0, True)
+    cache_close(got[~bad], want[~bad], dtype, max(np.abs(vq).max(), 5))
