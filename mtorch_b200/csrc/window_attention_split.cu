@@ -10,9 +10,10 @@
 //
 // Codes as operands: the 4 bits of a code at the low end of a 16-bit lane ARE the number c * 2^-133 in
 // bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly; at bits 4..7 they are 16 times that.  One
-// AND makes two operands, one shift serves half a word.  bf16 queries are multiplied by a power of two (exact), one
-// for the CTA's rows, that takes the largest finite value among them to 2^63..2^64: the products stay far from fp32's
-// own subnormals, and no value passes bf16's range.  Channels at bits 4..7 get a sixteenth.  With value = zero + scale c:
+// AND makes two operands, one shift serves half a word.  Queries are multiplied by a power of two (exact), one
+// for the CTA's rows, that takes the largest finite value among them to 2^63..2^64 in bf16 (the products stay far from
+// fp32's own subnormals, and no value passes bf16's range), to 2^14..2^15 in f16.  Channels at bits 4..7 get a sixteenth,
+// which costs an f16 value bits only where it is 2^24 below the largest.  With value = zero + scale c:
 //   q.k = scale (q.c) + zero sum(q)  per 64 channels,
 //   o   = sum (p scale) c + sum p zero,
 // with p scale rounded to bf16 (for f16 queries too, whose exponents are too few for p scale; they get the rounding's
@@ -309,7 +310,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
     }
   }
   // Q fragments (while the first keys are on their way): dense, 8 channels at 32 c + 8 t of row n; paged, the channel order of the codes' pairs
-  constexpr bool NORM = PAGED && !F16;  // rows multiplied by 2^kq
   uint32_t qf[NT][2 * DC][4];
   float qsum[NT][DC][2];
 #pragma unroll
@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
       for (int j = 0; j < 4; ++j) qf[x][c][j] = reinterpret_cast<const uint32_t*>(raw)[j];
     }
   }
-  int kq = 0;
-  if (NORM) {
+  int kq = 0;  // queries over codes are multiplied by 2^kq
+  if (PAGED) {
     constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
     uint32_t top2 = 0;
 #pragma unroll
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, DC * NT <= 2 ? (PAGED ? 4 : 
       for (int j = 0; j < 8; ++j) {
         v[j] = to_f32<T>(raw[j]);
         if (p.scale_log2 < 0.f) v[j] = -v[j];  // the maximum is taken of unscaled scores
-        if (NORM) v[j] = v[j] * q_up[0] * q_up[1];
+        if (PAGED) v[j] = v[j] * q_up[0] * q_up[1];
         const T h = from_f32<T>(PAGED && (j & 1) ? v[j] * 0.0625f : v[j]);
         u[j] = *reinterpret_cast<const uint16_t*>(&h);
       }

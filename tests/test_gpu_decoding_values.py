@@ -187,7 +187,8 @@ def cache_close(got, want, dtype, vmax):
 
 @pytest.mark.parametrize("H,Hkv,Sq,D,page", [(4, 2, 1, 64, 16), (8, 2, 3, 128, 32), (2, 2, 1, 256, 16), (12, 1, 2, 64, 64)])
 @pytest.mark.parametrize("dtype,power", [("bfloat16", 64), ("bfloat16", 90), ("bfloat16", 122), ("bfloat16", -60),
-                                         ("bfloat16", -90)])
+                                         ("bfloat16", -90), ("float16", -9), ("float16", -14), ("float16", -17),
+                                         ("float16", -21), ("float16", 11)])
 def test_cache_attention_of_small_and_large_queries(H, Hkv, Sq, D, page, dtype, power):
     """Queries near 2^power with a scale to match see what ordinary ones do; a head of them beside ordinary ones does too."""
     rng = np.random.default_rng(D + abs(power))
