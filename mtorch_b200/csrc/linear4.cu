@@ -9,10 +9,14 @@
 // end of a 16-bit lane are the number c * 2^-133 in bf16 (c * 2^-24 in f16), a subnormal that mma multiplies exactly,
 // at bits 4..7 sixteen times that: one AND makes two operands, one shift serves half a word.  The two places have
 // sums of their own (a sixteenth put on X instead would cost f16 values below 2^-10 their last bits).  X is laid out once
-// per CTA as operands in shared memory (bf16 times 2^64, to stay clear of fp32's subnormals), with the sums of -8 x
+// per CTA as operands in shared memory (bf16 times 2^80, to stay clear of fp32's subnormals), with the sums of -8 x
 // per row and group beside it, which take the codes' offset off: y += scale (low - 8 sum x + high / 16), in fp32 per
 // group of columns.  A warp brings its blocks of W with its own cp.async into a ring; no barrier stands between
 // the warps but at the end of a tile.
+//
+// Rows of X that this cannot hold, with an infinity, a NaN or (bf16, fp32) a largest value outside 2^-46..2^47, are
+// found while X is laid out; their outputs are summed up as they stand, a warp an output (w4_direct): infinity times a
+// weight is then what it has to be, and not NaN.  That takes many times as long.
 //
 // fp32 X goes as three bf16 parts (8 + 8 + 8 bits) in three rows of their own, added at the end.
 #include <algorithm>
@@ -66,13 +70,39 @@ __device__ __forceinline__ void w4_mma_zero(float (&d)[4], const uint32_t (&a)[4
 // Rows of the products that one row of X becomes.
 template <typename T> constexpr int w4_parts() { return sizeof(T) == 4 ? 3 : 1; }
 
-// A code counts c * 2^-24 in f16, c * 2^-133 in bf16 against operands scaled by 2^64.
+// A code counts c * 2^-24 in f16, c * 2^-133 in bf16 against operands scaled by 2^80.  (The scale leaves room on both
+// sides: X up to 2^47 fits, and weights and rows whose products are as small as 2^-73 do not underflow.)
 template <typename T>
 __device__ __forceinline__ constexpr float w4_unit() {
-  return std::is_same<T, __half>::value ? 16777216.f : 590295810358705651712.f;  // 2^24, 2^69
+  return std::is_same<T, __half>::value ? 16777216.f : 9007199254740992.f;  // 2^24, 2^53
 }
 
-// Eight columns of X as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7); bf16 times 2^64, f16 as it is.  `part`: which of the three bf16 parts of
+// Largest |x| of eight columns as bits of the type (of fp32: bits of fp32), a NaN above all.
+template <typename T>
+__device__ __forceinline__ uint32_t w4_top(const uint4 (&raw)[sizeof(T) / 2]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* v = reinterpret_cast<const T2*>(w);
+    const T2 m = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+    return max(u & 0x7fffu, u >> 16 & 0x7fffu);
+  }
+}
+// whether a row of this largest value has to be summed up as it stands
+template <typename T>
+__device__ __forceinline__ bool w4_odd(uint32_t top) {
+  if (std::is_same<T, __half>::value) return top >= 0x7c00u;
+  constexpr int sh = sizeof(T) == 4 ? 23 : 7;
+  return top >= (127u + 47u) << sh || (top != 0 && top < (127u - 46u) << sh);
+}
+
+// Eight columns of X as operands: pairs (0, 4), (1, 5), (2, 6), (3, 7); bf16 times 2^80, f16 as it is.  `part`: which of the three bf16 parts of
 // fp32.  Returns -8 times the columns' sum in the operands' unit.
 template <typename T>
 __device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], int part, uint4& out) {
@@ -90,14 +120,14 @@ __device__ __forceinline__ float w4_operands(const uint4 (&raw)[sizeof(T) / 2], 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         __nv_bfloat162& v = *reinterpret_cast<__nv_bfloat162*>(&w[j]);
-        const __nv_bfloat16 f = __ushort_as_bfloat16(0x5f80);  // 2^64
+        const __nv_bfloat16 f = __ushort_as_bfloat16(0x6780);  // 2^80
         v = __hmul2(v, __nv_bfloat162(f, f));
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum += to_f32<T>(e[j]);
   } else {
-    constexpr float f = 18446744073709551616.f;  // 2^64
+    constexpr float f = 1208925819614629174706176.f;  // 2^80
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -128,8 +158,39 @@ struct W4Smem {
   static __host__ __device__ int red(int rows) { return 2 * WARPS * rows * (16 * MT + 4) * 4; }
   static __host__ __device__ int ops(int rows, int Kp) { return rows * pitch(Kp); }
   static __host__ __device__ int sums(int Kp) { return Kp / GROUP * 8 * NT * 4; }
-  static __host__ __device__ int total(int rows, int Kp) { return red(rows) + WARPS * RING + ops(rows, Kp) + sums(Kp); }
+  static __host__ __device__ int total(int rows, int Kp) { return red(rows) + WARPS * RING + ops(rows, Kp) + sums(Kp) + 16; }
 };
+
+// Eight columns of a row x of X from column k on, zeros past K.
+template <typename T>
+__device__ __forceinline__ void w4_load8(const T* x, int k, int K, bool vec, uint4 (&raw)[sizeof(T) / 2]) {
+  const T* src = x + k;
+  if (vec && k + 8 <= K) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+  } else {
+    T* e = reinterpret_cast<T*>(raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = k + j < K ? src[j] : from_f32<T>(0.f);
+  }
+}
+
+// sum of x w over a row of X and a row of W by one warp, in fp32
+template <typename T, int GROUP>
+__device__ __noinline__ float w4_direct(const T* x, const uint32_t* words, const __nv_bfloat16* scales, int K, bool vec) {
+  float v = 0.f;
+  for (int i = threadIdx.x & 31; i * 8 < K; i += 32) {
+    uint4 raw[sizeof(T) / 2];
+    w4_load8<T>(x, i * 8, K, vec, raw);
+    const T* e = reinterpret_cast<const T*>(raw);
+    const uint32_t word = __ldg(words + (i & ~15) + w4_place(i & 15));
+    const float s = __bfloat162float(scales[i * 8 / GROUP]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i * 8 + j < K) v = fmaf(to_f32<T>(e[j]), s * (float)((int)(word >> (4 * j) & 15u) - 8), v);
+  }
+  return warp_sum(v);
+}
 
 // A CTA takes a run of strips of 16 rows of W (outputs), the same number for all but a strip, and goes through them MT at
 // a time against up to 8 * NT operand rows; its warps take blocks of 128 columns in turn and add up in shared memory.
@@ -148,6 +209,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
   uint8_t* ring = w4_smem + Smem::red(rows) + warp * Smem::RING;
   uint8_t* ops = w4_smem + Smem::red(rows) + WARPS * Smem::RING;
   float* sums = reinterpret_cast<float*>(ops + Smem::ops(rows, p.Kp));  // [group][8 NT]
+  uint32_t* odd_smem = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(sums) + Smem::sums(p.Kp));
   const uint32_t ring_u32 = smem_u32(ring);
   const int pitch_x = Smem::pitch(p.Kp);
   const int strips = (p.N + 15) / 16;
@@ -204,6 +266,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
   // X's operands: a warp takes 32 chunks of 8 columns of a row at a time (a group's chunks are neighbouring lanes)
   const int chunks = p.Kp / 8, segs = (chunks + 31) / 32, tasks = rows * segs;
   constexpr int U = 4;  // loads in flight
+  bool odd = false;
   for (int task0 = warp; task0 < tasks; task0 += U * WARPS) {
     uint4 raw[U][sizeof(T) / 2];
     int row[U], ch[U];
@@ -212,20 +275,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
       const int task = min(task0 + u * WARPS, tasks - 1);
       row[u] = task / segs;
       ch[u] = (task - row[u] * segs) * 32 + lane;
-      const int k = ch[u] * 8;
-      const T* src = static_cast<const T*>(p.x) + (int64_t)(row[u] / PARTS) * p.ldx + k;
-      if (p.x_vec && k + 8 <= p.K) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[u][i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      } else {
-        T* e = reinterpret_cast<T*>(raw[u]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = k + j < p.K ? src[j] : from_f32<T>(0.f);
-      }
+      w4_load8<T>(static_cast<const T*>(p.x) + (int64_t)(row[u] / PARTS) * p.ldx, ch[u] * 8, p.K, p.x_vec, raw[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint4 o;
+      odd |= w4_odd<T>(w4_top<T>(raw[u]));
       float sum = w4_operands<T>(raw[u], row[u] % PARTS, o);
 #pragma unroll
       for (int d = 1; d < GROUP / 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -235,7 +290,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
       }
     }
   }
-  __syncthreads();
+  uint32_t odd_rows = 0;  // bit m: row m is summed up as it stands
+  if (__syncthreads_or(odd)) {  // eight columns of some row: look at whole rows
+    if (threadIdx.x == 0) *odd_smem = 0;
+    __syncthreads();
+    for (int m = warp; m < p.M; m += WARPS) {
+      uint32_t top = 0;
+      for (int c = lane; c < chunks; c += 32) {
+        uint4 raw[sizeof(T) / 2];
+        w4_load8<T>(static_cast<const T*>(p.x) + (int64_t)m * p.ldx, c * 8, p.K, p.x_vec, raw);
+        top = max(top, w4_top<T>(raw));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0 && w4_odd<T>(top)) atomicOr(odd_smem, 1u << m);
+    }
+    __syncthreads();
+    odd_rows = *odd_smem;
+  }
 
   const uint8_t* xrow[NT];  // this lane's operand rows (rows past the last repeat it; their sums are not stored)
 #pragma unroll
@@ -337,7 +408,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
     __syncthreads();
     for (int i = threadIdx.x; i < p.M * OUT; i += WARPS * 32) {
       const int m = i / OUT, c = i % OUT;
-      if (n0 + c > last_row) continue;
+      if (n0 + c > last_row || (odd_rows >> m & 1u)) continue;
       float v = 0.f;
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
@@ -346,6 +417,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) linear4_kernel(const Linear4Par
       v *= w4_unit<T>();
       if (p.bias) v += to_f32<T>(static_cast<const T*>(p.bias)[n0 + c]);
       static_cast<T*>(p.y)[(int64_t)m * p.ldy + n0 + c] = from_f32<T>(v);
+    }
+    for (uint32_t left = odd_rows; left; left &= left - 1) {
+      const int m = __ffs(left) - 1;
+      for (int c = warp; c < OUT && n0 + c <= last_row; c += WARPS) {
+        const int64_t n = n0 + c;
+        float v = w4_direct<T, GROUP>(static_cast<const T*>(p.x) + (int64_t)m * p.ldx, p.words + n * (p.Kp / 8),
+                                      p.scales + n * (p.Kp / GROUP), p.K, p.x_vec);
+        if (p.bias) v += to_f32<T>(static_cast<const T*>(p.bias)[n0 + c]);
+        if (lane == 0) static_cast<T*>(p.y)[(int64_t)m * p.ldy + n0 + c] = from_f32<T>(v);
+      }
     }
     buf ^= 1;
     n0 += OUT;

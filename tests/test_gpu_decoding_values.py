@@ -222,3 +222,52 @@ def test_cache_attention_of_an_infinite_query(dtype):
     assert np.isnan(got[bad]).all() and bad.sum() == 2
     want = attention_ref(np.where(np.isfinite(qv), qv, 0), kq, vq, [126], [128], None, 0, True)
     cache_close(got[~bad], want[~bad], dtype, max(np.abs(vq).max(), 5))
+
+
+def product_close(got, x, w, dtype, add=0.0):
+    """Codes and 16-bit X multiply exactly; what is rounded are fp32 sums, of (code and 8) |x| scale <= 23 / 8 of the largest
+    |w| of a row times |x| over at most 24 additions of a group and its products (2^-23 each, 2^-18 together), and the result
+    to its type.  fp32 X goes in three parts that leave 2^-25."""
+    y = x @ w.T + add
+    mag = np.abs(x).sum(1)[:, None] * np.abs(w).max(1)[None] * (23 / 8)
+    lim = 2 * U[dtype] * np.abs(y) + 2.0 ** -18 * mag + 2.0 ** -24 * np.abs(add) + (2.0 ** -25 if dtype == "float16" else 0)
+    assert (np.abs(got - y) <= lim).all(), (np.abs(got - y) / lim).max()
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64)])
+@pytest.mark.parametrize("dtype,power", [("bfloat16", 64), ("bfloat16", 110), ("bfloat16", -70), ("float32", 64),
+                                         ("float32", 100), ("float32", -35), ("float32", -60)])
+def test_products_of_very_large_and_small_rows(M, N, K, group, dtype, power):
+    """Rows near 2^power, alone and among ordinary ones (the weights' scales keep the results in range)."""
+    rng = np.random.default_rng(M + abs(power))
+    p = mt.Weight4.pack(rounded(rng.standard_normal((N, K)) * 2.0 ** (-power // 2), "float32")[0], group)
+    w = host(p.unpack("float32"))
+    xn = rng.standard_normal((M, K))
+    xn[::2] *= 2.0 ** power
+    x, xv = rounded(xn, dtype)
+    product_close(host(mt.linear_weight4(x, p)), xv, w, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64)])
+def test_products_of_infinities_and_nan(M, N, K, group, dtype):
+    """As the definition has it: an infinity times a weight, NaN times a weight of zero and of infinities of both signs;
+    the other rows do not notice."""
+    rng = np.random.default_rng(M)
+    p = mt.Weight4.pack(rounded(rng.standard_normal((N, K)), "float32")[0], group)
+    w = host(p.unpack("float32"))
+    xn = rng.standard_normal((M, K))
+    rows = np.arange(M) % 4
+    xn[rows == 0, 5] = np.inf
+    xn[rows == 1, K - 1] = -np.inf
+    xn[rows == 2, 7] = np.nan
+    bias, bv = rounded(rng.standard_normal(N), dtype)
+    x, xv = rounded(xn, dtype)
+    got = host(mt.linear_weight4(x, p, bias))
+    with np.errstate(invalid="ignore"):
+        y = np.stack([(r[None] * w).sum(1) for r in xv]) + bv
+    fine = np.isfinite(y)
+    np.testing.assert_array_equal(got[~fine], y[~fine])
+    if M > 3:
+        assert fine.any() and np.isinf(y).any() and np.isnan(y).any()
+        product_close(got[rows == 3], xv[rows == 3], w, dtype, bv)
