@@ -478,8 +478,10 @@ int mt_cuda_kv_cache4_attention(const mt_kv_cache4_attention_desc* desc, void* w
  * the code of column c is in bits 4 (c % 8) of word c / 8, and in each 16 words (128 columns) word
  * w is stored at place (w % 4) * 4 + w / 4.  scales: [N, Kp / group] bf16, group 32, 64 or 128.
  * Codes of columns past K are ignored.  X and Y have row pitches, unit column stride; f32, bf16 or
- * f16, sums in fp32.  Workspace: mt_cuda_linear_weight4_workspace_size (many rows go through an
- * unpacked copy of the weight and mt_cuda_gemm).
+ * f16.  The weights enter exactly, whatever the type and number of rows; sums are fp32, rounded once
+ * to the type.  Infinities and NaN in X give what the definition gives.  Workspace:
+ * mt_cuda_linear_weight4_workspace_size (many rows go through f16 copies of the weight and of X, each row
+ * times a power of two, and mt_cuda_gemm).
  */
 typedef struct {
   int64_t M, N, K, group;

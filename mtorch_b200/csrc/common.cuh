@@ -332,6 +332,10 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+__device__ __forceinline__ float pow2_f32(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
+// x 2^n for |n| <= 252: a product with each half, so that neither factor leaves fp32's range
+__device__ __forceinline__ float ldexp_f32(float x, int n) { return x * pow2_f32(n >> 1) * pow2_f32(n - (n >> 1)); }
+
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

@@ -61,6 +61,8 @@ struct EpiParams {
   // TMA-store epilogue of a plain GEMM: the residual is read through a tensor map (32 x 32 boxes,
   // 64-byte swizzle, passed in the tmAlo slot) into the output staging buffers, a tile ahead
   int res_tma;
+  // run_gemm_shifted: D = A B^T 2^-(row_shift[m] + col_shift[n]) + bias (NULL: none)
+  const int* row_shift; const int* col_shift;
 };
 
 // 256-bit global accesses (sm_100): one instruction covers a whole 32-byte sector, so a warp whose
@@ -122,6 +124,18 @@ __device__ __forceinline__ void epi_gelu32(float (&v)[32], const float (&g)[32])
       v[j] *= a;
       v[j + 1] *= b;
     }
+  }
+}
+
+// 32 consecutive values of one row times 2^-(row + col[j]) (col has entries for whole groups of 32 columns)
+__device__ __forceinline__ void row_shift32(int row, const int* col, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const int4 c = __ldg(reinterpret_cast<const int4*>(col + j));
+    v[j] = ldexp_f32(v[j], min(max(-row - c.x, -252), 252));
+    v[j + 1] = ldexp_f32(v[j + 1], min(max(-row - c.y, -252), 252));
+    v[j + 2] = ldexp_f32(v[j + 2], min(max(-row - c.z, -252), 252));
+    v[j + 3] = ldexp_f32(v[j + 3], min(max(-row - c.w, -252), 252));
   }
 }
 
@@ -741,6 +755,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = ep.alpha * __uint_as_float(r[j]);
+            if (!CONV && !TF32 && ep.row_shift)
+              row_shift32(valid ? ep.row_shift[i1] : 0, ep.col_shift + col0, v);
             if (ep.bias)
               row_load_add(ep.bias, ep.bias_dtype, i0 * ep.bias_bstride + col0, nvalid, ep.bias_vec != 0, 1.f, v);
             if (ep.C && valid) row_load_add(ep.C, ep.out_dtype, offC + col0, nvalid, vec, ep.beta, v);
@@ -1236,6 +1252,11 @@ size_t gemm_workspace(const mt_gemm_desc& d) {
 }
 
 int run_gemm(const mt_gemm_desc& d, void* wsp, size_t ws_bytes, cudaStream_t st) {
+  return run_gemm_shifted(d, nullptr, nullptr, wsp, ws_bytes, st);
+}
+
+int run_gemm_shifted(const mt_gemm_desc& d, const int* row_shift, const int* col_shift, void* wsp, size_t ws_bytes,
+                     cudaStream_t st) {
   int rc = validate_gemm(d);
   if (rc) return rc;
   if (d.M == 0 || d.N == 0) return MT_OK;
@@ -1281,6 +1302,7 @@ int run_gemm(const mt_gemm_desc& d, void* wsp, size_t ws_bytes, cudaStream_t st)
   ep.res = d.residual; ep.r_s0 = d.stride_r; ep.r_s1 = d.ldr; ep.r_s2 = 0;
   ep.bias = d.bias; ep.bias_dtype = d.bias_dtype; ep.bias_bstride = d.bias_batch_stride;
   ep.alpha = d.alpha; ep.act = d.epilogue;
+  ep.row_shift = row_shift; ep.col_shift = col_shift;
   const int oes = dtype_size(d.out_dtype);
   bool vec = aligned16(d.D) && (d.ldd * oes) % 16 == 0 && (d.batch == 1 || (d.stride_d * oes) % 16 == 0);
   if (ep.C) vec = vec && aligned16(d.C) && (d.ldc * oes) % 16 == 0 && (d.batch == 1 || (d.stride_c * oes) % 16 == 0);

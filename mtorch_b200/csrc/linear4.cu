@@ -491,6 +491,99 @@ __global__ void __launch_bounds__(256) weight4_unpack_kernel(T* w, int64_t ldw, 
   }
 }
 
+// ---- many rows: products of f16 copies on the tensor-core GEMM ----
+//
+// scale * (code - 8) has at most 8 + 3 significant bits, which f16 holds and bf16 does not, and bf16 X fits f16's 11 bits
+// too.  Only the ranges differ: each row of W and of X is multiplied by a power of two that takes its largest finite value
+// near the top of f16's range, and the GEMM's epilogue takes the fp32 sums back by both.  What stands 2^28 (W) or 2^21
+// (X) below its row's largest value is rounded to 2^-40 of that.  fp32 X goes in two parts of 11 bits (what is left is
+// 2^-24 of a value): x1 and 2^11 x2 side by side, against w and 2^-11 w.
+// So the same row gives the same sums here and in linear4_kernel up to their order.
+
+// the power of two that takes the largest finite |x| of `bits` (fp32, as unsigned) to 2^to .. 2^(to + 1)
+__device__ __forceinline__ int w4_shift(uint32_t bits, int to) { return to + 127 - (int)(bits >> 23); }
+
+struct W4CopyParams {
+  Linear4Params p;
+  __half *wh, *xh;              // [N, parts * Kp], [M, parts * Kp]
+  int *row_shift, *col_shift;   // [M], [N]
+  int w_blocks;                 // CTAs that copy W, eight rows each; the others copy a row of X each
+};
+
+// Zeros past K in both.
+template <typename T>
+__global__ void __launch_bounds__(256) linear4_copy_kernel(const W4CopyParams c) {
+  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+  __shared__ uint32_t tops[8];
+  const Linear4Params& p = c.p;
+  const int W = p.Kp / 8;
+  if (blockIdx.x < c.w_blocks) {  // a warp per row of W
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (n >= p.N) return;
+    const __nv_bfloat16* sc = p.scales + n * (p.Kp / p.group);
+    uint32_t top = 0;
+    for (int i = lane; i * p.group < p.K; i += 32) {
+      const uint32_t u = __float_as_uint(__bfloat162float(sc[i])) & 0x7fffffffu;
+      if (u < 0x7f800000u) top = max(top, u);
+    }
+    const int b = w4_shift(__reduce_max_sync(0xffffffffu, top), 11);  // 8 scale: at most 2^15
+    if (lane == 0) c.col_shift[n] = b;
+    uint4* out = reinterpret_cast<uint4*>(c.wh) + n * PARTS * W;
+#pragma unroll 4
+    for (int i = lane; i < W; i += 32) {
+      const uint32_t word = __ldg(p.words + n * W + (i & ~15) + w4_place(i & 15));
+      const float s = ldexp_f32(__bfloat162float(sc[i * 8 / p.group]), b);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i * 8 + j < p.K ? s * (float)((int)(word >> (4 * j) & 15u) - 8) : 0.f;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        out[part * W + i] = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= 1.f / 2048.f;
+      }
+    }
+    return;
+  }
+  const int64_t m = blockIdx.x - c.w_blocks;
+  const T* row = static_cast<const T*>(p.x) + m * p.ldx;
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i * 8 < p.K; i += 256) {
+    uint4 raw[sizeof(T) / 2];
+    w4_load8<T>(row, i * 8, p.K, p.x_vec, raw);
+    const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t u = __float_as_uint(to_f32<T>(e[j])) & 0x7fffffffu;
+      if (u < 0x7f800000u) top = max(top, u);
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+  const int a = w4_shift(top, 14);
+  if (threadIdx.x == 0) c.row_shift[m] = a;
+  uint4* out = reinterpret_cast<uint4*>(c.xh) + m * PARTS * W;
+  for (int i = threadIdx.x; i < W; i += 256) {
+    uint4 raw[sizeof(T) / 2];
+    w4_load8<T>(row, i * 8, p.K, p.x_vec, raw);
+    const T* e = reinterpret_cast<const T*>(raw);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = ldexp_f32(to_f32<T>(e[j]), a);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      out[part * W + i] = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)  // (an infinity or NaN stands in the first part)
+        v[j] = isfinite(v[j]) ? (v[j] - __half2float(__float2half_rn(v[j]))) * 2048.f : 0.f;
+    }
+  }
+}
+
 static int64_t w4_padded(int64_t K) { return (K + 127) / 128 * 128; }
 
 static int w4_check(int64_t N, int64_t K, int64_t group, int dtype, const char* what) {
@@ -503,7 +596,7 @@ static int w4_check(int64_t N, int64_t K, int64_t group, int dtype, const char* 
 }
 
 // Rows and columns of X that go through linear4_kernel (the operands of one row, three for fp32, have to fit the shared
-// memory); others go through an unpacked copy of W and the tensor-core GEMM.
+// memory); others go through f16 copies and the tensor-core GEMM.
 constexpr int64_t kW4MaxRows = 64, kW4MaxCols = 16384;
 static bool w4_few(const mt_linear_weight4_desc& d) { return d.M <= kW4MaxRows && d.K <= kW4MaxCols; }
 
@@ -579,39 +672,63 @@ static int validate_linear4(const mt_linear_weight4_desc& d) {
   return MT_OK;
 }
 
-// Unpacked weight rows: a pitch of 16-byte multiples for the GEMM's tensor maps.
-static int64_t w4_pitch(const mt_linear_weight4_desc& d) { return (d.K + 7) / 8 * 8; }
-
-static mt_gemm_desc w4_gemm(const mt_linear_weight4_desc& d, void* w) {
+// Memory of the products of many rows: f16 copies of W and X and their rows' shifts.
+struct W4Many {
+  size_t w, x, row_shift, col_shift, gemm, total;
+};
+static mt_gemm_desc w4_gemm(const mt_linear_weight4_desc& d, const W4Many& w, char* ws) {
   mt_gemm_desc g{};
-  g.M = d.M; g.N = d.N; g.K = d.K; g.batch = 1;
-  g.dtype = g.out_dtype = d.dtype;
-  g.A = d.x; g.lda = d.ldx;
-  g.B = w; g.ldb = w4_pitch(d); g.b_trans = 1;
+  g.M = d.M; g.N = d.N; g.K = w4_padded(d.K) * (d.dtype == MT_F32 ? 2 : 1); g.batch = 1;
+  g.dtype = MT_F16; g.out_dtype = d.dtype;
+  g.A = ws + w.x; g.lda = g.K;
+  g.B = ws + w.w; g.ldb = g.K; g.b_trans = 1;
   g.D = d.y; g.ldd = d.ldy;
   g.bias = d.bias; g.bias_dtype = d.dtype;
   g.alpha = 1.f;
   return g;
 }
-static size_t w4_copy_bytes(const mt_linear_weight4_desc& d) {
-  return align_up((size_t)d.N * w4_pitch(d) * dtype_size(d.dtype), 1024);
+static W4Many w4_many(const mt_linear_weight4_desc& d) {
+  W4Many m{};
+  const size_t row = (size_t)w4_padded(d.K) * (d.dtype == MT_F32 ? 4 : 2);  // bytes of a row of a copy
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at = align_up(at + bytes, 1024);
+    return here;
+  };
+  m.w = take((size_t)d.N * row);
+  m.x = take((size_t)d.M * row);
+  m.row_shift = take((size_t)d.M * 4);
+  m.col_shift = take(align_up((size_t)d.N, 32) * 4);
+  m.gemm = at;
+  m.total = at + gemm_workspace(w4_gemm(d, m, reinterpret_cast<char*>(1024)));
+  return m;
+}
+
+template <typename T>
+static int linear4_many(const mt_linear_weight4_desc& d, const Linear4Params& p, char* ws, size_t ws_bytes, cudaStream_t st) {
+  const W4Many w = w4_many(d);
+  W4CopyParams c{};
+  c.p = p;
+  c.wh = reinterpret_cast<__half*>(ws + w.w);
+  c.xh = reinterpret_cast<__half*>(ws + w.x);
+  c.row_shift = reinterpret_cast<int*>(ws + w.row_shift);
+  c.col_shift = reinterpret_cast<int*>(ws + w.col_shift);
+  c.w_blocks = (p.N + 7) / 8;
+  if ((int64_t)c.w_blocks + d.M > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "linear_weight4: too many rows");
+  linear4_copy_kernel<T><<<(unsigned)(c.w_blocks + p.M), 256, 0, st>>>(c);
+  int rc = check_launch("linear_weight4 copies");
+  return rc ? rc : run_gemm_shifted(w4_gemm(d, w, ws), c.row_shift, c.col_shift, ws + w.gemm, ws_bytes - w.gemm, st);
 }
 
 size_t linear_weight4_workspace(const mt_linear_weight4_desc& d) {
-  if (validate_linear4(d) || w4_few(d) || d.N == 0 || d.K == 0) return 0;
-  return w4_copy_bytes(d) + gemm_workspace(w4_gemm(d, reinterpret_cast<void*>(1024)));
+  if (validate_linear4(d) || w4_few(d) || d.M == 0 || d.N == 0 || d.K == 0) return 0;
+  return w4_many(d).total;
 }
 
 int run_linear_weight4(const mt_linear_weight4_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
   int rc = validate_linear4(d);
   if (rc || d.M == 0 || d.N == 0) return rc;
-  if (!w4_few(d) && d.K > 0) {
-    if (!ws || ws_bytes < linear_weight4_workspace(d)) return fail(MT_ERR_WORKSPACE, "linear_weight4: workspace too small");
-    rc = run_weight4_unpack(ws, d.dtype, w4_pitch(d), d.words, d.scales, d.N, d.K, d.group, st);
-    if (rc) return rc;
-    const size_t copy = w4_copy_bytes(d);
-    return run_gemm(w4_gemm(d, ws), static_cast<char*>(ws) + copy, ws_bytes - copy, st);
-  }
   Linear4Params p{};
   p.M = (int)d.M; p.N = (int)d.N; p.K = (int)d.K; p.Kp = (int)w4_padded(d.K); p.group = (int)d.group;
   p.x = d.x; p.ldx = d.ldx;
@@ -619,6 +736,15 @@ int run_linear_weight4(const mt_linear_weight4_desc& d, void* ws, size_t ws_byte
   p.words = reinterpret_cast<const uint32_t*>(d.words);
   p.scales = static_cast<const __nv_bfloat16*>(d.scales);
   p.bias = d.bias; p.y = d.y; p.ldy = d.ldy;
+  if (!w4_few(d) && d.K > 0) {
+    if (!ws || ws_bytes < linear_weight4_workspace(d)) return fail(MT_ERR_WORKSPACE, "linear_weight4: workspace too small");
+    char* mem = static_cast<char*>(ws);
+    switch (d.dtype) {
+      case MT_F32: return linear4_many<float>(d, p, mem, ws_bytes, st);
+      case MT_BF16: return linear4_many<__nv_bfloat16>(d, p, mem, ws_bytes, st);
+      default: return linear4_many<__half>(d, p, mem, ws_bytes, st);
+    }
+  }
   switch (d.dtype) {
     case MT_F32: return linear4_run<float>(p, st);
     case MT_BF16: return linear4_run<__nv_bfloat16>(p, st);

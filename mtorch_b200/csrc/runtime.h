@@ -88,6 +88,10 @@ int launch_group_norm_cat(void* y, int yd, const int64_t* ys, const void* x1, co
                           cudaStream_t st);
 size_t gemm_workspace(const mt_gemm_desc& d);
 int run_gemm(const mt_gemm_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+// D = A B^T 2^-(row_shift[m] + col_shift[n]) + bias: shifts in device memory, col_shift 16-byte aligned and as long as N
+// rounded up to 32 (16-bit operands, one batch, no other epilogue)
+int run_gemm_shifted(const mt_gemm_desc& d, const int* row_shift, const int* col_shift, void* ws, size_t ws_bytes,
+                     cudaStream_t st);
 size_t conv_workspace(const mt_conv2d_desc& d);
 int run_conv2d(const mt_conv2d_desc& d, void* ws, size_t ws_bytes, cudaStream_t st);
 size_t conv_cat_workspace(const mt_conv2d_desc& d, const void* x2, const int64_t* x2_strides, int64_t c1);

@@ -391,7 +391,7 @@ class Weight4:
 
 def linear_weight4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tensor | None = None) -> Tensor:
     """`linear` with a weight held in 4 bits: x [..., cols] -> [..., out].  Made for few rows (a decoder's step);
-    many rows go through an unpacked copy of the weight and the tensor-core product."""
+    many rows go through copies in f16 (exact, rows of both times powers of two) and the tensor-core product."""
     what = "linear_weight4"
     _require_cuda(x, bias)
     _same_dtype(x, bias, what=what) if bias is not None else _same_dtype(x, what=what)

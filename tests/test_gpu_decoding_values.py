@@ -234,7 +234,8 @@ def product_close(got, x, w, dtype, add=0.0):
     assert (np.abs(got - y) <= lim).all(), (np.abs(got - y) / lim).max()
 
 
-@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64)])
+@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64),
+                                         (70, 40, 300, 64), (200, 130, 520, 32)])
 @pytest.mark.parametrize("dtype,power", [("bfloat16", 64), ("bfloat16", 110), ("bfloat16", -70), ("float32", 64),
                                          ("float32", 100), ("float32", -35), ("float32", -60)])
 def test_products_of_very_large_and_small_rows(M, N, K, group, dtype, power):
@@ -249,7 +250,8 @@ def test_products_of_very_large_and_small_rows(M, N, K, group, dtype, power):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
-@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64)])
+@pytest.mark.parametrize("M,N,K,group", [(1, 70, 96, 32), (3, 2400, 520, 64), (13, 70, 1000, 128), (33, 40, 300, 64),
+                                         (70, 50, 300, 64)])
 def test_products_of_infinities_and_nan(M, N, K, group, dtype):
     """As the definition has it: an infinity times a weight, NaN times a weight of zero and of infinities of both signs;
     the other rows do not notice."""
@@ -271,3 +273,22 @@ def test_products_of_infinities_and_nan(M, N, K, group, dtype):
     if M > 3:
         assert fine.any() and np.isinf(y).any() and np.isnan(y).any()
         product_close(got[rows == 3], xv[rows == 3], w, dtype, bv)
+
+
+@pytest.mark.parametrize("dtype,weights,rows", [("float16", -30, 12), ("float16", 18, -14), ("float16", 0, 0), ("bfloat16", -50, 0),
+                                                ("bfloat16", 60, -20), ("bfloat16", 0, 0), ("float32", -30, 10),
+                                                ("float32", 50, -20), ("float32", 0, 0)])
+@pytest.mark.parametrize("N,K,group", [(130, 200, 32), (70, 1000, 128)])
+def test_a_row_gives_the_same_in_a_prompt(N, K, group, dtype, weights, rows):
+    """64 rows, the same and one more, and many: the weights enter exactly in all of them, with scales past f16's range and
+    of many sizes too."""
+    rng = np.random.default_rng(abs(weights) + N)
+    wn = rng.standard_normal((N, K)) * 2.0 ** weights * 2.0 ** rng.integers(-6, 1, (N, 1))
+    p = mt.Weight4.pack(rounded(wn, "float32")[0], group)
+    w = host(p.unpack("float32"))
+    x, xv = rounded(rng.standard_normal((300, K)) * 2.0 ** rows / np.sqrt(K), dtype)
+    bias, bv = rounded(rng.standard_normal(N) * 2.0 ** (weights + rows), dtype)
+    for M in (1, 64, 65, 300):
+        product_close(host(mt.linear_weight4(x[:M], p, bias)), xv[:M], w, dtype, bv)
+    same = mt.linear_weight4(x[:1].expand(150, K), p, bias)  # one row in memory
+    product_close(host(same), np.repeat(xv[:1], 150, 0), w, dtype, bv)
