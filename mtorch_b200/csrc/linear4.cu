@@ -595,11 +595,6 @@ static int w4_check(int64_t N, int64_t K, int64_t group, int dtype, const char* 
   return MT_OK;
 }
 
-// Rows and columns of X that go through linear4_kernel (the operands of one row, three for fp32, have to fit the shared
-// memory); others go through f16 copies and the tensor-core GEMM.
-constexpr int64_t kW4MaxRows = 64, kW4MaxCols = 16384;
-static bool w4_few(const mt_linear_weight4_desc& d) { return d.M <= kW4MaxRows && d.K <= kW4MaxCols; }
-
 constexpr int kW4Smem = 227 * 1024;
 
 // Operand rows that fit a CTA of this shape.
@@ -608,6 +603,38 @@ static int w4_fit(int Kp) {
   using Smem = W4Smem<GROUP, MT, NT, WARPS>;
   const int left = kW4Smem - Smem::total(0, Kp);
   return left <= 0 ? 0 : std::min(8 * NT, left / (Smem::red(1) + Smem::ops(1, Kp)));
+}
+
+// Rows of X that a launch takes at most, 0 where not even one fits: one strip at a time but where every SM has two and the
+// registers allow it (up to 8 operand rows): X's operands are then read once for both.
+struct W4Fit {
+  int one, two, four, most;  // by NT
+};
+template <int GROUP>
+static W4Fit w4_fits(int Kp, int N, int parts) {
+  W4Fit f{};
+  f.one = (N > 16 * num_sms() ? w4_fit<GROUP, 2, 1, 16>(Kp) : w4_fit<GROUP, 1, 1, 16>(Kp)) / parts;
+  f.two = w4_fit<GROUP, 1, 2, 16>(Kp) / parts;
+  f.four = w4_fit<GROUP, 1, 4, 8>(Kp) / parts;
+  f.most = std::max(f.one, std::max(f.two, f.four));
+  return f;
+}
+
+// linear4_kernel, which reads W once a launch, or copies and the GEMM?  Up to two launches, three (fp32: four) where W has
+// 2^26 values: a launch then takes longer than what the other way costs beside its bytes.  Launches against copies, us,
+// 16-bit rows: 768 -> 2304, 32 / 64 rows (1 / 2 launches) 9 and 16 / 17 and 16; 4096 -> 4096, 32 / 48 (2 / 3) 30 and 40 /
+// 44 and 40; 5000 -> 4099, 32 / 48 (2 / 3) 49 and 54 / 73 and 54; 8192 -> 28672, 16 / 32 (2 / 4) 108 and 243 / 276 and 241;
+// 28672 -> 8192, 1 / 4 / 8 (1 / 2 / 4) 34 and 322 / 75 and 278 / 276 and 279.  fp32: 4096 -> 4096, 16 (3) 81 and 62;
+// 28672 -> 8192, 4 / 8 (4 / 8) 408 and 501 / 814 and 501.
+static bool w4_few(const mt_linear_weight4_desc& d) {
+  const int64_t Kp = w4_padded(d.K);
+  const int parts = d.dtype == MT_F32 ? 3 : 1;
+  if (Kp > kW4Smem) return false;  // (one row's operands take 2 bytes a column)
+  const int most = (d.group == 32   ? w4_fits<32>((int)Kp, (int)d.N, parts)
+                    : d.group == 64 ? w4_fits<64>((int)Kp, (int)d.N, parts)
+                                    : w4_fits<128>((int)Kp, (int)d.N, parts)).most;
+  const int64_t launches = d.N * Kp < (1 << 26) ? 2 : d.dtype == MT_F32 ? 4 : 3;
+  return d.M <= launches * most;
 }
 
 template <typename T, int GROUP, int MT, int NT, int WARPS>
@@ -635,20 +662,14 @@ static int linear4_launch(const Linear4Params& p, int rows_x, cudaStream_t st) {
   return MT_OK;
 }
 
-// Rows of X a launch: as many as fit the shared memory, evenly over the launches.  One strip at a time but where every SM
-// has two and the registers allow it (up to 8 operand rows): X's operands are then read once for both.
+// Rows of X are shared out evenly over the launches.
 template <typename T, int GROUP>
 static int linear4_dispatch(const Linear4Params& p, cudaStream_t st) {
-  constexpr int PARTS = w4_parts<T>();
-  const bool two = p.N > 16 * num_sms();
-  const int fit1 = (two ? w4_fit<GROUP, 2, 1, 16>(p.Kp) : w4_fit<GROUP, 1, 1, 16>(p.Kp)) / PARTS;
-  const int fit2 = w4_fit<GROUP, 1, 2, 16>(p.Kp) / PARTS, fit4 = w4_fit<GROUP, 1, 4, 8>(p.Kp) / PARTS;
-  const int most = std::max(fit1, std::max(fit2, fit4));
-  if (most < 1) return fail(MT_ERR_UNSUPPORTED, "linear_weight4: %d columns do not fit the shared memory", p.K);
-  const int launches = (p.M + most - 1) / most, rows = (p.M + launches - 1) / launches;
-  if (rows <= fit1)
-    return two ? linear4_launch<T, GROUP, 2, 1, 16>(p, rows, st) : linear4_launch<T, GROUP, 1, 1, 16>(p, rows, st);
-  if (rows <= fit2) return linear4_launch<T, GROUP, 1, 2, 16>(p, rows, st);
+  const W4Fit f = w4_fits<GROUP>(p.Kp, p.N, w4_parts<T>());
+  const int launches = (p.M + f.most - 1) / f.most, rows = (p.M + launches - 1) / launches;
+  if (rows <= f.one)
+    return p.N > 16 * num_sms() ? linear4_launch<T, GROUP, 2, 1, 16>(p, rows, st) : linear4_launch<T, GROUP, 1, 1, 16>(p, rows, st);
+  if (rows <= f.two) return linear4_launch<T, GROUP, 1, 2, 16>(p, rows, st);
   return linear4_launch<T, GROUP, 1, 4, 8>(p, rows, st);
 }
 

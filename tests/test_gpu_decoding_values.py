@@ -4,10 +4,13 @@ very small numbers in the decoder's operators, against 64-bit references.
 The forms of `window_attention` are reached by shape and type: "tc" and "tiles" by many queries, "split" and "rows" by few
 (`path_of` asserts which).
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import mtorch_b200 as mt
+from mtorch_b200 import _lib as L
 from test_gpu_decoding import U, attention_ref, heads, host, i32, path_of, quantised, rounded
 
 pytestmark = pytest.mark.gpu
@@ -292,3 +295,30 @@ def test_a_row_gives_the_same_in_a_prompt(N, K, group, dtype, weights, rows):
         product_close(host(mt.linear_weight4(x[:M], p, bias)), xv[:M], w, dtype, bv)
     same = mt.linear_weight4(x[:1].expand(150, K), p, bias)  # one row in memory
     product_close(host(same), np.repeat(xv[:1], 150, 0), w, dtype, bv)
+
+
+def products_in_one_read(M, N, K, group, dtype):
+    """Whether `linear_weight4` reads the packed weight itself (it needs no workspace then)."""
+    code = mt.zeros(1, dtype=dtype).dtype.code
+    d = L.LinearWeight4Desc(M, N, K, group, code, 16, K, 16, 16, None, 16, N)
+    return L.lib().mt_cuda_linear_weight4_workspace_size(C.byref(d)) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("N,K,group", [(70, 768, 64), (40, 4096, 128), (33, 17000, 32), (20, 28672, 128)])
+def test_products_on_both_sides_of_the_switch(N, K, group, dtype):
+    """Where the copies take over from the packed weight, by type and columns; a few rows of a wide weight never go through
+    them."""
+    rows = [M for M in range(1, 200) if products_in_one_read(M, N, K, group, dtype)]
+    last = rows[-1]
+    assert rows == list(range(1, last + 1)) and 1 <= last < 199
+    rng = np.random.default_rng(K)
+    p = mt.Weight4.pack(rounded(rng.standard_normal((N, K)), "float32")[0], group)
+    w = host(p.unpack("float32"))
+    x, xv = rounded(rng.standard_normal((last + 1, K)) / np.sqrt(K), dtype)
+    for M in {1, last, last + 1}:
+        got = host(mt.linear_weight4(x[:M], p))
+        y = xv[:M] @ w.T
+        # (sums over more additions than product_close has: K / 16 of them within 2^-23 of the sum of |x w|)
+        lim = 2 * U[dtype] * np.abs(y) + (2.0 ** -18 * 8 + K / 16 * 2.0 ** -23) * (np.abs(xv[:M]) @ np.abs(w).T)
+        assert (np.abs(got - y) <= lim + (2.0 ** -25 if dtype == "float16" else 0)).all()
