@@ -16,7 +16,7 @@ def test_few_rows_of_a_wide_weight_need_no_copy(group):
     """One token of a projection from 28672 columns is read from the packed weight, not through a copy of four times its size."""
     for dtype in (L.MT_BF16, L.MT_F16):
         assert reads_packed_weight(1, 8192, 28672, group, dtype)
-    assert reads_packed_weight(1, 8192, 28672 if group == 128 else 24576, group, L.MT_F32)  # (three operand rows)
+    assert reads_packed_weight(1, 8192, 28672 if group == 128 else 20480, group, L.MT_F32)  # (three operand rows)
     assert reads_packed_weight(4, 8192, 28672, group, L.MT_BF16)
 
 
