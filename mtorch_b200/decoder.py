@@ -17,19 +17,52 @@ import numpy as np
 
 from . import decoding, ops
 from .nn import LayerNorm, Linear, Module, ModuleList, init
-from .tensor import _new, empty, tensor
+from .tensor import Tensor, _new, empty, tensor
 
 
 class Linear4(Module):
-    """`Linear` with the weight held in 4 bits (`decoding.Weight4`): packed from a floating `Linear`."""
+    """`Linear` with the weight held in 4 bits (`decoding.Weight4`): packed from a floating `Linear`.  Its parameters are
+    the packed `words` and `scales`, whose types stay whatever the module is cast to, and the bias; a state dict
+    with a floating `weight` in their place is packed as it is loaded."""
 
     def __init__(self, linear: Linear, group: int = 64):
         super().__init__()
-        self.weight4 = decoding.Weight4.pack(linear.weight, group)
+        self.cols, self.group = linear.in_features, group
+        w = decoding.Weight4.pack(linear.weight, group)
+        self.register_parameter("words", w.words)
+        self.register_parameter("scales", w.scales)
         self.register_parameter("bias", linear.bias)
+        self._weight4 = w
+
+    @property
+    def weight4(self) -> decoding.Weight4:
+        w = self._weight4
+        if w.words is not self.words or w.scales is not self.scales:  # moved since
+            w = self._weight4 = decoding.Weight4(self.words, self.scales, self.cols)
+        return w
 
     def forward(self, x):
         return decoding.linear_weight4(x, self.weight4, self.bias)
+
+    def _apply(self, fn):
+        words, scales = self.words, self.scales
+        self._parameters.update(words=None, scales=None)
+        super()._apply(fn)
+        dev = (self.bias if self.bias is not None else fn(scales)).device
+        self.register_parameter("words", words.to(dev))
+        self.register_parameter("scales", scales.to(dev))
+        return self
+
+    def _load_other(self, key, value):
+        if key != "weight":
+            return super()._load_other(key, value)
+        value = value if isinstance(value, Tensor) else tensor(value)
+        if tuple(value.shape) != (self.words.shape[0], self.cols):
+            raise ValueError(f"Linear4: weight {list(value.shape)}, expected {[self.words.shape[0], self.cols]}")
+        w = decoding.Weight4.pack(value.to(self.words.device), self.group)
+        self.words.copy_(w.words)
+        self.scales.copy_(w.scales)
+        return True
 
 
 class DecoderLayer(Module):
@@ -93,8 +126,15 @@ class Decoder(Module):
         init.normal_(self.token_embedding, 0.0, 0.02)
         self.layers = ModuleList([DecoderLayer(width, heads, kv_heads, mlp, group, device, dtype) for _ in range(layers)])
         self.final_norm = LayerNorm(width, device=device, dtype=dtype)
-        self.frequencies = decoding.rotary_frequencies(self.sections, device=device)
+        self.register_buffer("frequencies", decoding.rotary_frequencies(self.sections, device=device))
         self._state = None
+
+    def _apply(self, fn):
+        f = self.frequencies
+        self._buffers["frequencies"] = None
+        super()._apply(fn)
+        self.register_buffer("frequencies", f.to(self.token_embedding.device))  # (float32 whatever the module is cast to)
+        return self
 
     def start(self, batch: int, tokens: int) -> None:
         """Makes room for `batch` sequences of up to `tokens` tokens: a cache per layer and the table of pages."""

@@ -82,9 +82,14 @@ class Module:
         for k, v in sd.items():
             if k in own:
                 own[k].copy_(v)
-            elif strict:
+            elif not self._load_other(k, v) and strict:
                 raise KeyError(f"unexpected key {k}")
         return self
+
+    def _load_other(self, key, value) -> bool:
+        """Takes an entry of a state dict that is no parameter here (a module that holds its weight in another form)."""
+        name, _, rest = key.partition(".")
+        return bool(rest) and name in self._modules and self._modules[name]._load_other(rest, value)
 
     def _apply(self, fn):
         for n, p in list(self._parameters.items()):
