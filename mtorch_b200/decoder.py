@@ -9,7 +9,7 @@ the text goes on behind the largest of them.  Attention sees a sliding window an
 
 A prompt runs through `window_attention` on its own keys and values and is then appended to the cache
 (`prefill`); each further token is appended and attends over the cache (`step`), two calls a layer beside the
-projections.
+projections.  In float32 a step reads the cache back first.
 """
 from __future__ import annotations
 
@@ -17,7 +17,7 @@ import numpy as np
 
 from . import decoding, ops
 from .nn import LayerNorm, Linear, Module, ModuleList, init
-from .tensor import Tensor, _new, empty, tensor
+from .tensor import Tensor, _new, empty, float32, tensor, zeros
 
 
 class Linear4(Module):
@@ -94,6 +94,9 @@ class DecoderLayer(Module):
         decoding.kv_cache_append(cache, k, v, state.table, state.starts)
         if state.prompt:
             decoding.window_attention(q, k, v, state.window, state.sinks, out=av)
+        elif h.dtype is float32:  # (the cache's attention takes 16-bit queries)
+            k, v = decoding.kv_cache_read(cache, state.table, state.zeros, state.capacity, dtype=float32)
+            decoding.window_attention(q, k, v, state.window, state.sinks, starts=state.starts, lengths=state.lengths, out=av)
         else:
             decoding.kv_cache_attention(q, cache, state.table, state.lengths, window=state.window, sinks=state.sinks,
                                         out=av)
@@ -145,6 +148,7 @@ class Decoder(Module):
         st.caches = [decoding.KVCache4.empty(batch * per, self.page_size, self.kv_heads, self.dim, device=dev)
                      for _ in self.layers]
         st.table = tensor(np.arange(batch * per, dtype=np.int32).reshape(batch, per), dtype="int32").to(dev)
+        st.zeros = zeros(batch, dtype="int32", device=dev)
         st.frequencies, st.sections, st.window, st.sinks = self.frequencies, self.sections, self.window, self.sinks
         st.count = st.place = 0  # tokens so far; the next text token's position
 

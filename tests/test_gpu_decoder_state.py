@@ -5,6 +5,7 @@ import pytest
 import mtorch_b200 as mt
 from mtorch_b200 import nn
 from mtorch_b200.decoder import Decoder, Linear4
+from test_gpu_decoder import TOL, forward, host, place
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,19 @@ def test_a_floating_weight_is_packed_as_it_is_loaded():
     w = mt.tensor(rng.standard_normal((128, 96)).astype(np.float32) * 0.1)
     m.load_state_dict({"layers.1.fc2.weight": w})
     np.testing.assert_array_equal(m.layers[1].fc2.words.numpy(), mt.Weight4.pack(w.cuda(), 64).words.numpy())
+
+
+def test_float32_prompt_and_steps():
+    """Steps follow a prompt in float32 too."""
+    mt.manual_seed(7)
+    model = Decoder(vocab=90, width=128, layers=2, heads=2, kv_heads=1, mlp=96, window=20, sinks=2, page_size=16, dtype="float32")
+    n, s, steps = 2, 30, 4
+    ids = np.random.default_rng(0).integers(0, 90, (n, s + steps))
+    want = forward(model, host(model.token_embedding)[ids], place(0, 0, s + steps), s)
+    model.start(n, s + steps)
+    got = [host(model.prefill(mt.tensor(ids[:, :s])))]
+    for i in range(steps):
+        got.append(host(model.step(mt.tensor(ids[:, s + i]))))
+    for i, g in enumerate(got):
+        assert np.abs(g - want[:, s - 1 + i]).max() <= TOL * np.abs(want).max(), i
+    assert model.generate(mt.tensor(ids[:, :s]), 3).shape == (n, 3)
