@@ -238,7 +238,7 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   p.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
   p.num_pages = (int)c.num_pages;
   p.Hkv = (int)c.Hkv; p.D = (int)c.D; p.T = (int)T;
-  if (B > 65535 || T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
+  if (T * c.Hkv > INT32_MAX / 64) return fail(MT_ERR_UNSUPPORTED, "%s: too many tokens", what);
   p.items = (int)((T + tokens - 1) / tokens * c.Hkv * (c.D / 8));
   p.starts = starts;
   p.by_words = FastDiv((uint32_t)(c.D / 8));
@@ -255,6 +255,14 @@ static int cache4_params(Cache4Params& p, const mt_kv_cache4& c, const void* k, 
   return MT_OK;
 }
 
+// Sequences stand in the grid's second axis, larger batches in several launches: the one from sequence b on.
+constexpr int64_t kMaxGridY = 65535;
+static dim3 cache4_grid(Cache4Params& p, int64_t b, int64_t B, const int32_t* table, const int32_t* starts) {
+  p.table = table ? table + b * p.table_stride : nullptr;
+  p.starts = starts + b;
+  return dim3((unsigned)((p.items + 255) / 256), (unsigned)std::min(B - b, kMaxGridY));
+}
+
 int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
                          int dtype, int64_t B, int64_t T, const int32_t* table, int64_t table_stride,
                          int64_t max_pages, const int32_t* starts, cudaStream_t st) {
@@ -262,15 +270,20 @@ int run_kv_cache4_append(const mt_kv_cache4& c, const void* k, const int64_t* ks
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, kAppendTokens,
                          "kv_cache4_append");
   if (rc || B == 0 || p.items == 0) return rc;
-  p.in[0] = k; p.in[1] = v;
   p.by_inner = FastDiv((uint32_t)c.Hkv);
-  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)B);
-  switch (dtype) {
-    case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
-    case MT_BF16: cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
-    default: cache4_append_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+  const int64_t es = dtype_size(dtype);
+  for (int64_t b = 0; b < B && !rc; b += kMaxGridY) {
+    p.in[0] = static_cast<const char*>(k) + b * ks[0] * es;
+    p.in[1] = static_cast<const char*>(v) + b * vs[0] * es;
+    const dim3 grid = cache4_grid(p, b, B, table, starts);
+    switch (dtype) {
+      case MT_F32: cache4_append_kernel<float><<<grid, 256, 0, st>>>(p); break;
+      case MT_BF16: cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
+      default: cache4_append_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+    }
+    rc = check_launch("kv_cache4_append");
   }
-  return check_launch("kv_cache4_append");
+  return rc;
 }
 
 int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* v, const int64_t* vs, int dtype,
@@ -280,15 +293,20 @@ int run_kv_cache4_read(const mt_kv_cache4& c, void* k, const int64_t* ks, void* 
   int rc = cache4_params(p, c, k, ks, v, vs, dtype, B, T, table, table_stride, max_pages, starts, kReadTokens,
                          "kv_cache4_read");
   if (rc || B == 0 || p.items == 0) return rc;
-  p.out[0] = k; p.out[1] = v;
   p.by_inner = FastDiv((uint32_t)((T + kReadTokens - 1) / kReadTokens));
-  dim3 grid((unsigned)((p.items + 255) / 256), (unsigned)B);
-  switch (dtype) {
-    case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;
-    case MT_BF16: cache4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
-    default: cache4_read_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+  const int64_t es = dtype_size(dtype);
+  for (int64_t b = 0; b < B && !rc; b += kMaxGridY) {
+    p.out[0] = static_cast<char*>(k) + b * ks[0] * es;
+    p.out[1] = static_cast<char*>(v) + b * vs[0] * es;
+    const dim3 grid = cache4_grid(p, b, B, table, starts);
+    switch (dtype) {
+      case MT_F32: cache4_read_kernel<float><<<grid, 256, 0, st>>>(p); break;
+      case MT_BF16: cache4_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p); break;
+      default: cache4_read_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+    }
+    rc = check_launch("kv_cache4_read");
   }
-  return check_launch("kv_cache4_read");
+  return rc;
 }
 
 }  // namespace mt

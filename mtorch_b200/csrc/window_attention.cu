@@ -557,8 +557,53 @@ int window_attention_path(const mt_window_attention_desc& d) {
                       : takes_tiles(d) ? MT_WINDOW_PATH_TILES : MT_WINDOW_PATH_ROWS;
 }
 
+// The kernels of few rows have a (batch entry, key head) in the grid's second axis: larger batches go in parts.
+constexpr int64_t kMaxBatchHeads = 65535;
+static int64_t batch_part(int64_t B, int64_t Hkv) { return std::min(B, std::max<int64_t>(1, kMaxBatchHeads / Hkv)); }
+
+static mt_window_attention_desc batch_from(const mt_window_attention_desc& d, int64_t b, int64_t n) {
+  mt_window_attention_desc p = d;
+  const int64_t es = dtype_size(d.dtype);
+  auto at = [&](const void* base, const int64_t* st) { return static_cast<const char*>(base) + b * st[0] * es; };
+  p.B = n;
+  if (d.starts) p.starts = d.starts + b;
+  if (d.lengths) p.lengths = d.lengths + b;
+  p.q = at(d.q, d.q_strides);
+  p.o = const_cast<char*>(at(d.o, d.o_strides));
+  if (d.k) p.k = at(d.k, d.k_strides);
+  if (d.v) p.v = at(d.v, d.v_strides);
+  return p;
+}
+static mt_kv_cache4_attention_desc batch_from(const mt_kv_cache4_attention_desc& d, int64_t b, int64_t n) {
+  mt_kv_cache4_attention_desc p = d;
+  p.B = n;
+  p.lengths = d.lengths + b;
+  if (d.block_table) p.block_table = d.block_table + b * d.table_stride;
+  p.q = static_cast<const char*>(d.q) + b * d.q_strides[0] * 2;
+  p.o = static_cast<char*>(d.o) + b * d.o_strides[0] * 2;
+  return p;
+}
+static bool in_parts(const mt_window_attention_desc& d) {
+  return batch_part(d.B, d.Hkv) < d.B && !takes_sm100(d) && (takes_split(d) || !takes_tiles(d));
+}
+static bool in_parts(const mt_kv_cache4_attention_desc& d) { return batch_part(d.B, d.cache.Hkv) < d.B; }
+
+// `run` on parts of `per` batch entries, the last one the rest; or the larger of the two parts' workspaces.
+template <typename Desc, typename Run>
+static int run_parts(const Desc& d, int64_t per, Run run) {
+  int rc = MT_OK;
+  for (int64_t b = 0; b < d.B && !rc; b += per) rc = run(batch_from(d, b, std::min(per, d.B - b)));
+  return rc;
+}
+template <typename Desc, typename Size>
+static size_t parts_workspace(const Desc& d, int64_t per, Size size) {
+  const int64_t rest = d.B % per;
+  return std::max(size(batch_from(d, 0, per)), rest ? size(batch_from(d, d.B - rest, rest)) : 0);
+}
+
 size_t window_attention_workspace(const mt_window_attention_desc& d) {
   if (validate_window(d) || d.B == 0 || d.Sq == 0) return 0;
+  if (in_parts(d)) return parts_workspace(d, batch_part(d.B, d.Hkv), window_attention_workspace);
   const int splits = window_splits(d);
   if (takes_split(d) && split_joins_in_cluster(d.B * d.Hkv, d.Sq * (d.H / d.Hkv), splits)) return 0;
   return part_bytes(splits, d.B * d.H * d.Sq, d.D);
@@ -589,6 +634,11 @@ static int window_dispatch(const mt_window_attention_desc& d, const AttnParams& 
 int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
   int rc = validate_window(d);
   if (rc || d.B == 0 || d.Sq == 0) return rc;
+  if (in_parts(d)) {
+    if (ws_bytes < window_attention_workspace(d)) return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
+    return run_parts(d, batch_part(d.B, d.Hkv),
+                     [&](const mt_window_attention_desc& p) { return run_window_attention(p, ws, ws_bytes, st); });
+  }
   AttnParams p{};
   p.B = (int)d.B; p.H = (int)d.H; p.Hkv = (int)d.Hkv; p.g = (int)(d.H / d.Hkv);
   p.Sq = (int)d.Sq; p.Sk = (int)d.Sk; p.D = (int)d.D; p.rows = p.g * p.Sq;
@@ -634,6 +684,7 @@ static int validate_cache_attention(const mt_kv_cache4_attention_desc& d) {
 
 size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d) {
   if (validate_cache_attention(d) || d.B == 0 || d.Sq == 0) return 0;
+  if (in_parts(d)) return parts_workspace(d, batch_part(d.B, d.cache.Hkv), kv_cache4_attention_workspace);
   const int splits = cache_splits(d);
   if (split_joins_in_cluster(d.B * d.cache.Hkv, d.Sq * (d.H / d.cache.Hkv), splits)) return 0;
   return part_bytes(splits, d.B * d.H * d.Sq, d.cache.D);
@@ -642,6 +693,11 @@ size_t kv_cache4_attention_workspace(const mt_kv_cache4_attention_desc& d) {
 int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
   int rc = validate_cache_attention(d);
   if (rc || d.B == 0 || d.Sq == 0) return rc;
+  if (in_parts(d)) {
+    if (ws_bytes < kv_cache4_attention_workspace(d)) return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
+    return run_parts(d, batch_part(d.B, d.cache.Hkv),
+                     [&](const mt_kv_cache4_attention_desc& p) { return run_kv_cache4_attention(p, ws, ws_bytes, st); });
+  }
   AttnParams p{};
   p.B = (int)d.B; p.H = (int)d.H; p.Hkv = (int)d.cache.Hkv; p.g = (int)(d.H / d.cache.Hkv);
   p.Sq = (int)d.Sq; p.Sk = (int)(d.max_pages * d.cache.page_size); p.D = (int)d.cache.D; p.rows = p.g * p.Sq;
