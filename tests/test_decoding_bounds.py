@@ -4,6 +4,8 @@ u = 2^-9 for bf16, 2^-12 for f16, 2^-25 for fp32 (half a step of rounding).
 * f16 queries over the 4-bit cache: the weights times scale go to bf16 in two parts, which leaves 2^-18 of them, against codes
   of -8..7: 2^-18 of 8 scale, below 2^-17 of the largest |v| (or 5) here; scores of fp32 sums move the result by at most 1e-4 of
   that; the result is rounded.
+* 16-bit attention of few queries: the weights go to their 16-bit type in two parts, which leaves 2^-18 of them (bf16, less in
+  f16): 2^-17 of the largest |v|, scores move the result by at most 1e-4 of it; the result is rounded.
 * products of fp32 rows with 4-bit weights: X goes in three parts of 8 bits.  Where all of X lies between 1 and 2, the codes'
   sums of 16 products are whole multiples of 2^-23 below 2^9 in each part and exact in fp32 (a part has 8 bits, a code 4, 16 of them 4 more);
   what is rounded are the sums over groups (4 to a block of 128 columns), over blocks and the parts: below 8 roundings of 2^-24
@@ -88,6 +90,53 @@ def test_the_cache_bound_sees_weights_of_one_part(case, parts):
             rest = (e * (zero[b, hk, :, g] + 8 * scale[b, hk, :, g])).sum(1, keepdims=True)
             got[b, h][:, g * 64:(g + 1) * 64] = (r @ (code[b, hk, :, g] - 8) + rest) / total
     off = np.abs(got.astype(np.float16).astype(np.float64) - want) > cache_limit(want, vq)
+    assert off.any() == (parts == 1)
+
+
+SPLIT = [
+    # dtype, H, Hkv, Sq, Sk, D, window
+    ("bfloat16", 4, 2, 1, 60, 64, 5),
+    ("bfloat16", 8, 1, 2, 300, 128, 12),
+    ("bfloat16", 6, 2, 4, 900, 64, 900),
+    ("bfloat16", 16, 2, 2, 500, 256, 8),
+    ("float16", 4, 2, 1, 60, 64, 5),
+    ("float16", 8, 1, 2, 300, 128, 12),
+]
+
+
+def split_limit(want, vv, dtype):
+    return 2 * U[dtype] * np.abs(want) + (2.0 ** -17 + 1e-4) * np.abs(vv).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,H,Hkv,Sq,Sk,D,window", SPLIT)
+def test_16_bit_attention_of_few_queries(dtype, H, Hkv, Sq, Sk, D, window):
+    rng = np.random.default_rng(Sk + D)
+    q, qv = heads(rng, 2, H, Sq, D, dtype)
+    k, kv = heads(rng, 2, Hkv, Sk, D, dtype)
+    v, vv = heads(rng, 2, Hkv, Sk, D, dtype)
+    assert path_of(q, k, v, window, 0) == "split"
+    got = host(mt.window_attention(q, k, v, window))
+    want = attention_ref(qv, kv, vv, [Sk - Sq] * 2, [Sk] * 2, window, 0, True)
+    assert (np.abs(got - want) <= split_limit(want, vv, dtype)).all()
+
+
+@pytest.mark.parametrize("parts", [1, 2])
+@pytest.mark.parametrize("dtype,H,Hkv,Sq,Sk,D,window", [c for c in SPLIT if c[0] == "bfloat16" and c[6] < 100])
+def test_the_attention_bound_sees_weights_of_one_part(dtype, H, Hkv, Sq, Sk, D, window, parts):
+    rng = np.random.default_rng(Sk + D)
+    q, k, v = (bf16(rng.standard_normal((2, h, s, D))) for h, s in ((H, Sq), (Hkv, Sk), (Hkv, Sk)))
+    want = attention_ref(q, k, v, [Sk - Sq] * 2, [Sk] * 2, window, 0, True)
+    got = np.zeros_like(want)
+    for b, h in itertools.product(range(2), range(H)):
+        m = sees((Sk - Sq + np.arange(Sq))[:, None], np.arange(Sk)[None], Sk, window, 0, True)
+        s = np.where(m, q[b, h] @ k[b, h * Hkv // H].T / np.sqrt(D), -np.inf)
+        e = np.exp(s - s.max(1, keepdims=True))
+        w = bf16(e)
+        if parts == 2:
+            w = w + bf16(e - w)
+        got[b, h] = w @ v[b, h * Hkv // H] / e.sum(1, keepdims=True)
+    off = np.abs(bf16(got) - want) > split_limit(want, v, dtype)
     assert off.any() == (parts == 1)
 
 
