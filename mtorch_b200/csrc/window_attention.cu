@@ -399,9 +399,13 @@ static int64_t span_keys(int64_t Sk, int64_t Sq, int causal, int64_t window, int
   return std::min(Sk, (causal ? window : 2 * window - 1) + Sq - 1 + sinks + 2 * kRowBlock);
 }
 
-// Shares of the keys: enough CTAs to fill the GPU a few times, each with at least 8 blocks of keys.
-static int choose_splits(int64_t ctas, int64_t keys) {
-  const int64_t want = (4LL * num_sms() + ctas - 1) / ctas;
+// Shares of the keys: enough CTAs to fill the GPU a few times, each with at least 8 blocks of keys.  A step of few tokens (one
+// tile of rows a key head) is cut finer, more rows pay more for the join.  fp32, us with 2, 4 and 8 CTAs an SM: one token of
+// 8 sequences, 32 / 8 heads of 128, window 4096: 105, 115, 107 (floor 41); of 24 sequences, 16 heads of 64, 4096 keys: 233, 240,
+// 193 (124); 2 / 8 heads, 30000 keys: 40, 37, 37; 32 queries of 4 x 16 heads, 500 keys, 4 and 8: 56, 60; 200 of 16 / 4 heads over
+// 4000 keys, window 1000: 194, 211.
+static int choose_splits(int64_t ctas, int64_t tiles, int64_t keys) {
+  const int64_t want = ((tiles == 1 ? 8LL : 4LL) * num_sms() + ctas - 1) / ctas;
   const int64_t most = std::max<int64_t>(1, keys / (8 * kRowBlock));
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), kMaxSplits));
 }
@@ -414,7 +418,7 @@ static size_t part_bytes(int splits, int64_t rows, int64_t D) {
 static int rows_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int causal, int64_t window,
                        int64_t sinks) {
   const int64_t tiles = (Sq * (H / Hkv) + kRowTile - 1) / kRowTile;
-  return choose_splits(B * Hkv * tiles, span_keys(Sk, Sq, causal, window, sinks));
+  return choose_splits(B * Hkv * tiles, tiles, span_keys(Sk, Sq, causal, window, sinks));
 }
 
 // Rows of head dim channels are whole 16-byte vectors of a 16-bit type.
@@ -444,11 +448,13 @@ static bool takes_sm100(const mt_window_attention_desc& d) {
   return tiles_us < split_us;
 }
 
-// fp32 (and what neither of the two takes): tiles of 64 queries where they make a third of the SMs busy, else rows with
-// the keys split.  Tiles and rows: 300 queries of 4 heads over 600 keys 78 and 41 us (20 tiles), of 16 heads 78 and 95
-// (80 tiles); 3 x 1500 of 16 heads 0.9 and 2.8 ms.
+// fp32 (and what neither of the two takes): tiles of 64 queries from 24 queries of a head an SM on, else rows with the keys
+// split.  Tiles and rows, us, by queries of all heads: 1200 (300 of 4 heads over 600 keys) 77 and 40; 2048 (32 of 4 x 16, 500)
+// 79 and 56; 3200 (200 of 16, 4000, window 1000) 216 and 194; 3600 (150 of 24, 300) 42 and 56; 4000 (2000 of 2, window 256) 42
+// and 49; 4160 (130 of 2 x 16, 1000) 154 and 161; 8704 (17 of 64 x 8, 1000, heads of 128) 631 and 667; 72000 (1500 of 3 x 16, 1500)
+// 541 and 1704.
 static bool takes_tiles(const mt_window_attention_desc& d) {
-  return d.Sq > 16 && d.B * d.H * ((d.Sq + kTile - 1) / kTile) * 3 >= num_sms();
+  return d.Sq > 16 && d.B * d.H * d.Sq >= 24 * num_sms();
 }
 
 static int window_splits(const mt_window_attention_desc& d) {
