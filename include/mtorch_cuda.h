@@ -369,6 +369,7 @@ int mt_cuda_sdpa(const mt_sdpa_desc* desc, void* workspace, size_t workspace_byt
 int mt_cuda_sdpa_path(const mt_sdpa_desc* desc);
 
 /* ---- a causal decoder's operators (no counterpart in the reference) ----------------------- */
+/* Workspaces of these calls have to be 16-byte aligned (MT_ERR_INVALID). */
 /*
  * Rotary positions with several axes (time, height, width, ...) on one or two tensors of heads.
  * Pair i of `pairs` turns by angle(i) = fp32(position[axis of i] * frequencies[i]); axis a owns the

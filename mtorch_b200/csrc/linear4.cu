@@ -759,6 +759,7 @@ int run_linear_weight4(const mt_linear_weight4_desc& d, void* ws, size_t ws_byte
   p.bias = d.bias; p.y = d.y; p.ldy = d.ldy;
   if (!w4_few(d) && d.K > 0) {
     if (!ws || ws_bytes < linear_weight4_workspace(d)) return fail(MT_ERR_WORKSPACE, "linear_weight4: workspace too small");
+    if ((uintptr_t)ws % 16) return fail(MT_ERR_INVALID, "linear_weight4: the workspace has to be 16-byte aligned");
     char* mem = static_cast<char*>(ws);
     switch (d.dtype) {
       case MT_F32: return linear4_many<float>(d, p, mem, ws_bytes, st);

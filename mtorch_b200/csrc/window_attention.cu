@@ -470,6 +470,14 @@ static int cache_splits(const mt_kv_cache4_attention_desc& d) {
                      span_keys(d.max_pages * d.cache.page_size, d.Sq, 1, d.window, d.sinks));
 }
 
+// The partial results are stored 16 bytes at a time.
+static int check_workspace(const void* ws, size_t bytes, size_t need, const char* what) {
+  if (!need) return MT_OK;
+  if (!ws || bytes < need) return fail(MT_ERR_WORKSPACE, "%s: workspace too small", what);
+  if ((uintptr_t)ws % 16) return fail(MT_ERR_INVALID, "%s: the workspace has to be 16-byte aligned", what);
+  return MT_OK;
+}
+
 static void bind_workspace(AttnParams& p, void* ws) {
   const size_t rows = (size_t)p.B * p.Hkv * p.rows;
   p.part_ml = static_cast<float2*>(ws);
@@ -641,7 +649,8 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
   int rc = validate_window(d);
   if (rc || d.B == 0 || d.Sq == 0) return rc;
   if (in_parts(d)) {
-    if (ws_bytes < window_attention_workspace(d)) return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
+    rc = check_workspace(ws, ws_bytes, window_attention_workspace(d), "window_attention");
+    if (rc) return rc;
     return run_parts(d, batch_part(d.B, d.Hkv),
                      [&](const mt_window_attention_desc& p) { return run_window_attention(p, ws, ws_bytes, st); });
   }
@@ -658,8 +667,8 @@ int run_window_attention(const mt_window_attention_desc& d, void* ws, size_t ws_
     p.qs[i] = d.q_strides[i]; p.ks[i] = d.k_strides[i]; p.vs[i] = d.v_strides[i]; p.os[i] = d.o_strides[i];
   }
   p.splits = window_splits(d);
-  const size_t need = window_attention_workspace(d);
-  if (need && (!ws || ws_bytes < need)) return fail(MT_ERR_WORKSPACE, "window_attention: workspace too small");
+  rc = check_workspace(ws, ws_bytes, window_attention_workspace(d), "window_attention");
+  if (rc) return rc;
   bind_workspace(p, ws);
   if (takes_sm100(d)) return run_window_sm100(d, p, st);
   if (takes_split(d)) {
@@ -700,7 +709,8 @@ int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size
   int rc = validate_cache_attention(d);
   if (rc || d.B == 0 || d.Sq == 0) return rc;
   if (in_parts(d)) {
-    if (ws_bytes < kv_cache4_attention_workspace(d)) return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
+    rc = check_workspace(ws, ws_bytes, kv_cache4_attention_workspace(d), "kv_cache4_attention");
+    if (rc) return rc;
     return run_parts(d, batch_part(d.B, d.cache.Hkv),
                      [&](const mt_kv_cache4_attention_desc& p) { return run_kv_cache4_attention(p, ws, ws_bytes, st); });
   }
@@ -724,8 +734,8 @@ int run_kv_cache4_attention(const mt_kv_cache4_attention_desc& d, void* ws, size
   p.num_pages = (int)d.cache.num_pages;
   p.page_shift = __builtin_ctzll((unsigned long long)d.cache.page_size);
   p.splits = cache_splits(d);
-  const size_t need = kv_cache4_attention_workspace(d);
-  if (need && (!ws || ws_bytes < need)) return fail(MT_ERR_WORKSPACE, "kv_cache4_attention: workspace too small");
+  rc = check_workspace(ws, ws_bytes, kv_cache4_attention_workspace(d), "kv_cache4_attention");
+  if (rc) return rc;
   bind_workspace(p, ws);
   p.q_vec = aligned16(d.q, d.q_strides, d.cache.D);
   rc = run_split_attention(p, d.dtype, true, st);

@@ -29,3 +29,20 @@ def test_many_launches_give_way_to_the_copy():
     assert reads_packed_weight(64, 2304, 768, 64, L.MT_BF16)
     assert not reads_packed_weight(65, 2304, 768, 64, L.MT_BF16)
     assert reads_packed_weight(100, 64, 0, 64, L.MT_BF16)  # (no columns: the bias alone)
+
+
+def test_a_workspace_off_its_alignment_is_refused():
+    """Partial results and copies are stored 16 bytes at a time: nothing is launched on a workspace that is not aligned."""
+    lib = L.lib()
+    st = (1 << 20, 1 << 14, 64, 1)
+    w = L.WindowAttentionDesc(1, 4, 2, 1, 8192, 64, L.MT_BF16, 1, 0, 0, None, None, 16, st, 16, st, 16, st, 16, st, 0.125)
+    need = lib.mt_cuda_window_attention_workspace_size(C.byref(w))
+    assert need and lib.mt_cuda_window_attention(C.byref(w), 8, need, None) == L.MT_ERR_INVALID
+    assert lib.mt_cuda_window_attention(C.byref(w), 16, need - 1, None) == L.MT_ERR_WORKSPACE
+    cache = L.KvCache4Desc(1024, 16, 2, 64, 16, 16, 16, 16)
+    c = L.KvCache4AttentionDesc(cache, 1, 4, 1, L.MT_BF16, 0, 0, 16, 1024, 1024, 16, 16, st, 16, st, 0.125)
+    need = lib.mt_cuda_kv_cache4_attention_workspace_size(C.byref(c))
+    assert need and lib.mt_cuda_kv_cache4_attention(C.byref(c), 8, need, None) == L.MT_ERR_INVALID
+    d = L.LinearWeight4Desc(500, 80, 256, 64, L.MT_BF16, 16, 256, 16, 16, None, 16, 80)
+    need = lib.mt_cuda_linear_weight4_workspace_size(C.byref(d))
+    assert need and lib.mt_cuda_linear_weight4(C.byref(d), 8, need, None) == L.MT_ERR_INVALID
