@@ -181,6 +181,13 @@ __device__ __forceinline__ uint32_t wa_elect() {
   return r;
 }
 
+// After a wait that expired: what this CTA has in flight may still land, so nothing leaves before it has, or a bound.
+__device__ __forceinline__ void wa_drain(uint64_t* bar, uint32_t parity) {
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - start < kWaitBudgetCycles / 8) {
+  }
+}
+
 template <int DP>
 struct WaCfg {
   static constexpr int TILE = kWaTile * DP * 2;  // bytes of a tile of Q, K or V
@@ -216,7 +223,8 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   uint64_t* s_full = v_empty + Cfg::STAGES_V;     // [2]
   uint64_t* p_full = s_full + 2;                  // [2][2]: the first and the second 64 keys of P_x
   uint64_t* o_done = p_full + 4;                  // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* mma_idle = o_done + 2;                // after an expired wait: the products issued so far are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_idle + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -255,6 +263,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
       mbar_init(&p_full[2 * x + 1], kWaTile);
       mbar_init(&o_done[x], 1);
     }
+    mbar_init(mma_idle, 1);
     *abort_flag = 0;
     fence_barrier_init();
     if (bl.count > 0) {  // Q and the first K tile come while the rest is set up
@@ -282,10 +291,13 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     int ks = 1, vs = 0;
     uint32_t kph = 0, vph = 0;
     bool ok = true;
+    int k_loads = bl.count > 0, v_loads = 0;  // so far, without the tile of V that is fixed (it can only be the last one)
+    bool raw_load = false;
     auto load_k = [&](int i) {
       if (lane == 0 && ok) {
         ok = mbar_wait(&k_empty[ks], kph ^ 1, 71, abort_flag);
         if (ok) {
+          ++k_loads;
           mbar_arrive_expect_tx(&k_full[ks], Cfg::TILE);
           for (int c = 0; c < CHUNKS; ++c)
             tma_load_4d(sK + ks * Cfg::TILE + c * Cfg::CHUNK, &tmK, &k_full[ks], c * 64, bl.block(i) * kWaTile, hk, b);
@@ -306,6 +318,8 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         ok = mbar_wait(&v_empty[vs], vph ^ 1, 72, abort_flag);
         if (ok) {
           uint64_t* bar = fix ? v_raw : &v_full[vs];
+          raw_load = fix;
+          v_loads += !fix;
           mbar_arrive_expect_tx(bar, Cfg::TILE);
           for (int c = 0; c < CHUNKS; ++c)
             tma_load_4d(sV + vs * Cfg::TILE + c * Cfg::CHUNK, &tmV, bar, c * 64, k0, hk, b);
@@ -326,6 +340,12 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         vs = 0;
         vph ^= 1;
       }
+    }
+    if (lane == 0 && *abort_flag && bl.count > 0) {
+      wa_drain(q_full, 0);
+      for (int n = max(0, k_loads - Cfg::STAGES_K); n < k_loads; ++n) wa_drain(&k_full[n % Cfg::STAGES_K], (n / Cfg::STAGES_K) & 1);
+      for (int n = max(0, v_loads - Cfg::STAGES_V); n < v_loads; ++n) wa_drain(&v_full[n % Cfg::STAGES_V], (n / Cfg::STAGES_V) & 1);
+      if (raw_load) wa_drain(v_raw, 0);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (the whole warp runs it, one lane issues) ----------------
@@ -402,6 +422,10 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         }
         a0 = n0;
         a1 = n1;
+      }
+      if (!ok || *abort_flag) {
+        wa_commit(mma_idle, leader);
+        wa_drain(mma_idle, 0);
       }
     }
   } else if (warp >= 4) {
