@@ -399,7 +399,9 @@ int mt_cuda_rotary(const mt_rotary_desc* desc, void* stream);
  * with n = lengths[b] (NULL: Sk; clamped to 0..Sk) it sees key j < n when
  *   causal:      j <= p and (window == 0 or j > p - window or j < sinks)
  *   otherwise:   window == 0 or |p - j| < window or j < sinks.
- * A query that sees nothing gets zeros.  Keys at n and beyond may hold anything.  Q [B, H, Sq, D],
+ * A query that sees nothing gets zeros.  Keys at n and beyond may hold anything; V below n has to be finite
+ * (a NaN or an infinity at a key can reach queries near those that see it), a NaN in a query or in the keys that
+ * it sees makes it NaN.  Q [B, H, Sq, D],
  * K and V [B, Hkv, Sk, D], O [B, H, Sq, D] with element strides (b, h, s, d), H % Hkv == 0,
  * D <= 256, Sq and Sk <= 2^28; f32, bf16, f16 (softmax and sums in fp32).  starts / lengths: int32 on
  * the device; starts are clamped to +-2^29.
@@ -457,7 +459,8 @@ int mt_cuda_kv_cache4_read(const mt_kv_cache4* cache, void* k_out, const int64_t
 /* Causal attention of the last Sq tokens of each sequence over the cache, with an optional window
  * and sinks as in mt_cuda_window_attention: query i of sequence b has position lengths[b] - Sq + i
  * and the sequence has lengths[b] keys (clamped to 0 .. max_pages * page_size).  q and o
- * [B, H, Sq, D] in bf16 or f16. */
+ * [B, H, Sq, D] in bf16 or f16 (any finite values: they are multiplied by a power of two of their own).  Tokens
+ * below the length that hold NaN can reach queries near those that see them. */
 typedef struct {
   mt_kv_cache4 cache;
   int64_t B, H, Sq;

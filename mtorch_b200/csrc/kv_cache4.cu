@@ -1,5 +1,5 @@
 // Writing to and reading from the paged 4-bit key / value cache (attention over it:
-// window_attention.cu).
+// window_attention_split.cu).
 //
 // One thread per word of 8 channels, 8 neighbouring threads per group of 64 channels: the group's
 // minimum and maximum come from three shuffles.  Bound by memory: the values are read once and 36
@@ -8,7 +8,7 @@
 
 namespace mt {
 
-// n / d for n < 2^31 by a multiplication (d >= 1): m = floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)
+// n / d for n < 2^31 by a multiplication (d >= 1; division by an invariant integer, Granlund and Montgomery 1994): m = floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)
 struct FastDiv {
   uint32_t d, m, s;
   FastDiv() = default;

@@ -1,5 +1,5 @@
-// Attention with a sliding window and sinks, over 16-bit / fp32 keys and values or over the paged
-// 4-bit cache.
+// Attention with a sliding window and sinks: the choice of the kernel (16-bit prompts: window_attention_sm100.cu; few queries
+// over 16-bit keys and over the 4-bit cache: window_attention_split.cu), the kernels in fp32, and the join of split keys.
 //
 // One pass over the keys with the running maximum and sum of the softmax in fp32:
 //   m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' = o 2^(m - m') + 2^(s - m') v.

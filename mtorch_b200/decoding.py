@@ -309,7 +309,8 @@ def kv_cache_attention(q: Tensor, cache: KVCache4, block_table: Tensor, lengths:
     """Causal attention of the last tokens of each sequence, `q` [B, H, Sq, dim] (bfloat16 or float16), over the
     cache: query i is at position lengths[b] - Sq + i and sees the keys up to itself, with `window` and
     `sinks` as in `window_attention`.  `lengths` int32 [B] counts the tokens in the cache, the queries' own
-    among them (append first).  H may be a multiple of the cache's heads."""
+    among them (append first).  Tokens below it that hold NaN can reach neighbouring queries that do not see them.  H may
+    be a multiple of the cache's heads."""
     what = "kv_cache_attention"
     _require_cuda(q, block_table, lengths)
     if q.dim() != 4 or q._shape[3] != cache.dim:
