@@ -680,7 +680,12 @@ def from_device_memory(ptr: int, shape, dtype, *, strides=None, device=0, owner=
         raise ValueError("from_device_memory: strides and shape have to be as many and not negative")
     if ptr % dt.itemsize or (ptr == 0 and math.prod(shape)):
         raise ValueError(f"from_device_memory: address {ptr:#x} for {dt.name}")
-    idx = int(getattr(device, "index", device) or 0)
+    if not isinstance(device, (int, np.integer)):
+        dev = globals()["device"](device)
+        if dev.type != "cuda":
+            raise ValueError(f"from_device_memory: {dev} is no cuda device")
+        device = dev.index or 0
+    idx = int(device)
     _ensure_device(idx)
     last = sum((n - 1) * s for n, s in zip(shape, strides)) if math.prod(shape) else -1
     return Tensor(_rt.ExternalBuffer(ptr, (last + 1) * dt.itemsize, idx, owner), 0, shape, strides, dt,
