@@ -620,12 +620,13 @@ static W4Fit w4_fits(int Kp, int N, int parts) {
   return f;
 }
 
-// linear4_kernel, which reads W once a launch, or copies and the GEMM?  Up to two launches, three (fp32: four) where W has
-// 2^26 values: a launch then takes longer than what the other way costs beside its bytes.  Launches against copies, us,
-// 16-bit rows: 768 -> 2304, 32 / 64 rows (1 / 2 launches) 9 and 16 / 17 and 16; 4096 -> 4096, 32 / 48 (2 / 3) 30 and 40 /
-// 44 and 40; 5000 -> 4099, 32 / 48 (2 / 3) 49 and 54 / 73 and 54; 8192 -> 28672, 16 / 32 (2 / 4) 108 and 243 / 276 and 241;
-// 28672 -> 8192, 1 / 4 / 8 (1 / 2 / 4) 34 and 322 / 75 and 278 / 276 and 279.  fp32: 4096 -> 4096, 16 (3) 81 and 62;
-// 28672 -> 8192, 4 / 8 (4 / 8) 408 and 501 / 814 and 501.
+// linear4_kernel, which reads W once a launch, or copies and the GEMM?  16-bit rows: up to two launches, three where W has 2^26
+// values.  fp32, whose copies are larger and go through the GEMM in passes: two, three from 2^22 and six from 2^26 values
+// on.  Launches against copies, us, 16-bit rows: 768 -> 2304, 32 / 64 rows (1 / 2 launches) 9 and 16 / 17 and 16; 4096 -> 4096,
+// 32 / 48 (2 / 3) 30 and 40 / 44 and 40; 5000 -> 4099, 32 / 48 (2 / 3) 49 and 54 / 73 and 54; 8192 -> 28672, 16 / 32 (2 / 4) 108
+// and 243 / 276 and 241; 28672 -> 8192, 1 / 4 / 8 (1 / 2 / 4) 34 and 322 / 75 and 278 / 276 and 279.  fp32: 768 -> 2304, 16 / 24
+// (2 / 3) 24 and 28 / 35 and 28; 4096 -> 4096, 16 / 24 (3 / 4) 81 and 92 / 116 and 93; 8192 -> 28672, 16 / 24 (6 / 8) 385 and 475 /
+// 525 and 485; 28672 -> 8192, 6 / 8 (6 / 8) 612 and 724 / 815 and 723.
 static bool w4_few(const mt_linear_weight4_desc& d) {
   const int64_t Kp = w4_padded(d.K);
   const int parts = d.dtype == MT_F32 ? 3 : 1;
@@ -633,7 +634,8 @@ static bool w4_few(const mt_linear_weight4_desc& d) {
   const int most = (d.group == 32   ? w4_fits<32>((int)Kp, (int)d.N, parts)
                     : d.group == 64 ? w4_fits<64>((int)Kp, (int)d.N, parts)
                                     : w4_fits<128>((int)Kp, (int)d.N, parts)).most;
-  const int64_t launches = d.N * Kp < (1 << 26) ? 2 : d.dtype == MT_F32 ? 4 : 3;
+  const int64_t values = d.N * Kp;
+  const int64_t launches = d.dtype == MT_F32 ? (values < (1 << 22) ? 2 : values < (1 << 26) ? 3 : 6) : values < (1 << 26) ? 2 : 3;
   return d.M <= launches * most;
 }
 
@@ -726,6 +728,8 @@ static W4Many w4_many(const mt_linear_weight4_desc& d) {
   return m;
 }
 
+constexpr int64_t kW4Pass = 1024;
+
 template <typename T>
 static int linear4_many(const mt_linear_weight4_desc& d, const Linear4Params& p, char* ws, size_t ws_bytes, cudaStream_t st) {
   const W4Many w = w4_many(d);
@@ -739,7 +743,25 @@ static int linear4_many(const mt_linear_weight4_desc& d, const Linear4Params& p,
   if ((int64_t)c.w_blocks + d.M > INT32_MAX) return fail(MT_ERR_UNSUPPORTED, "linear_weight4: too many rows");
   linear4_copy_kernel<T><<<(unsigned)(c.w_blocks + p.M), 256, 0, st>>>(c);
   int rc = check_launch("linear_weight4 copies");
-  return rc ? rc : run_gemm_shifted(w4_gemm(d, w, ws), c.row_shift, c.col_shift, ws + w.gemm, ws_bytes - w.gemm, st);
+  if (rc) return rc;
+  const mt_gemm_desc all = w4_gemm(d, w, ws);
+  if (d.dtype != MT_F32) return run_gemm_shifted(all, c.row_shift, c.col_shift, ws + w.gemm, ws_bytes - w.gemm, st);
+  // fp32: the tensor core's accumulator drops what does not fit in each step of 16 columns, which grows to 1e-5 of the
+  // result at 4000 columns.  So the second parts have sums of their own, and the first parts' columns go 1024 at a time; Y
+  // adds up the passes in fp32.
+  for (int64_t k = -1; k < p.Kp && !rc; k = k < 0 ? 0 : k + kW4Pass) {
+    mt_gemm_desc g = all;
+    const int64_t at = k < 0 ? p.Kp : k;
+    g.K = k < 0 ? p.Kp : std::min<int64_t>(kW4Pass, p.Kp - k);
+    g.A = static_cast<const __half*>(all.A) + at;
+    g.B = static_cast<const __half*>(all.B) + at;
+    if (k >= 0) {
+      g.bias = nullptr;
+      g.C = g.D; g.ldc = g.ldd; g.beta = 1.f;
+    }
+    rc = run_gemm_shifted(g, c.row_shift, c.col_shift, ws + w.gemm, ws_bytes - w.gemm, st);
+  }
+  return rc;
 }
 
 size_t linear_weight4_workspace(const mt_linear_weight4_desc& d) {

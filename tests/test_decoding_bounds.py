@@ -10,6 +10,8 @@ u = 2^-9 for bf16, 2^-12 for f16, 2^-25 for fp32 (half a step of rounding).
   sums of 16 products are whole multiples of 2^-23 below 2^9 in each part and exact in fp32 (a part has 8 bits, a code 4, 16 of them 4 more);
   what is rounded are the sums over groups (4 to a block of 128 columns), over blocks and the parts: below 8 roundings of 2^-24
   of sum |x w| for one block, 2^-21.
+* the same for many rows: 1024 columns are 64 steps of an accumulator that drops what does not fit, 2^-23 each at most: 2^-17
+  of sum |x w|, with a rounding of 2^-24 for each pass of 1024 columns.
 * attention in fp32: scores of D products are off by at most D 2^-24 sum |q k| scale, an exponential by 2^-22, sums over n keys by n 2^-24:
   together (D sum|q k| scale + n + 8) 2^-24 of the largest |v|.
 
@@ -162,6 +164,20 @@ def test_fp32_products_hold_fp32(M, N, group):
     xt, xv = rounded(x, "float32")
     np.testing.assert_array_equal(xv, x)
     assert (np.abs(host(mt.linear_weight4(xt, p)) - xv @ wv.T) <= product_limit(xv, wv)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,group", [(300, 130, 128, 64), (150, 70, 3449, 64), (100, 300, 8192, 128)])
+def test_fp32_products_of_many_rows_hold_fp32(M, N, K, group):
+    """All of one sign: what the accumulator drops does not cancel (without passes it grows to 2^-15 at 8192 columns)."""
+    rng = np.random.default_rng(K)
+    p = mt.Weight4.pack(rounded(np.abs(rng.standard_normal((N, K))) + 0.5, "float32")[0], group)
+    w = host(p.unpack("float32"))
+    x, xv = rounded(np.abs(rng.standard_normal((M, K))) + 0.5, "float32")
+    bias, bv = rounded(rng.standard_normal(N), "float32")
+    y = xv @ w.T
+    got = host(mt.linear_weight4(x, p, bias))
+    assert (np.abs(got - y - bv) <= (2.0 ** -17 + (K // 1024 + 3) * 2.0 ** -24) * y).all()
 
 
 @pytest.mark.parametrize("parts", [1, 2, 3])
