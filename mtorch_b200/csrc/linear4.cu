@@ -16,7 +16,8 @@
 //
 // Rows of X that this cannot hold, with an infinity, a NaN or (bf16, fp32) a largest value outside 2^-46..2^47, are
 // found while X is laid out; their outputs are summed up as they stand, a warp an output (w4_direct): infinity times a
-// weight is then what it has to be, and not NaN.  That takes many times as long.
+// weight is then what it has to be, and not NaN.  One such row of 8192 -> 28672 takes 174 us in the place of 40, 13 of
+// 5000 -> 4099 204 in the place of 20.
 //
 // fp32 X goes as three bf16 parts (8 + 8 + 8 bits) in three rows of their own, added at the end.
 #include <algorithm>
